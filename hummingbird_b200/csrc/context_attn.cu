@@ -1,0 +1,157 @@
+// C entry points of the context attention: argument checks, how a call is cut into work items, and its launches.
+#include <algorithm>
+#include <cmath>
+#include <cuda_runtime.h>
+
+#include "../../include/hb_b200.h"
+#include "abi_common.h"
+#include "context_attn.h"
+
+namespace hb {
+namespace {
+
+constexpr int kSms = 148;
+constexpr int kMaxSlots = 256;
+
+struct Shape {
+  int B, Lq, Lkv, Ls, H, Hkv, D;
+};
+
+struct Plan {
+  CtxPart part[2];
+  int slots;
+  int rows_per_tile;
+  size_t bytes;  // partial results
+};
+
+bool shape_ok(const Shape& s) {
+  if (s.B < 1 || s.Lq < 1 || s.Lkv < 0 || s.Ls < 0 || s.H < 1 || s.Hkv < 1 || s.H % s.Hkv) return false;
+  if (s.D != 64 && s.D != 128) return false;
+  // a kv head's rows over the whole batch, and the items of a call, are counted in 32 bits
+  const int64_t rows = (int64_t)s.B * s.Lq * s.H;
+  return rows < (1ll << 30) && s.Lkv < (1 << 30) && s.Ls < (1 << 30);
+}
+
+int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+
+// Parts of a list of `chunks` key chunks over `items` items: two CTAs for every SM where the list is long enough
+// to give each of a CTA's four warps two chunks.
+int splits_for(int64_t items, int chunks) {
+  const int want = ceil_div(2 * kSms, items);
+  return std::max(1, std::min(want, std::max(1, chunks / 8)));
+}
+
+Plan make_plan(const Shape& s) {
+  Plan p{};
+  const int G = s.H / s.Hkv, kc = 2048 / s.D;
+  const int rows = s.Lq * G;
+  const bool pooled = s.Ls > 0 && s.B > 1 && rows < 128;
+  const int rows0 = pooled ? rows * s.B : rows;
+  p.rows_per_tile = s.D == 64 && rows0 > 16 ? 32 : 16;
+  const int n_sh = ceil_div(s.Ls, kc), n_own = ceil_div(s.Lkv, kc);
+  auto fill = [&](CtxPart& part, bool pool, bool sh, bool own, int chunks, int part_rows) {
+    part.pooled = pool;
+    part.use_shared = sh;
+    part.use_own = own;
+    part.row_tiles = ceil_div(part_rows, p.rows_per_tile);
+    const int64_t items = (int64_t)(pool ? 1 : s.B) * s.Hkv * part.row_tiles;
+    part.splits = std::min(splits_for(items, chunks), kMaxSlots / 2);
+    part.slot0 = p.slots;
+    part.ctas = static_cast<int>(items * part.splits);
+    p.slots += part.splits;
+  };
+  if (pooled) {
+    fill(p.part[0], true, true, false, n_sh, rows0);
+    if (s.Lkv > 0) fill(p.part[1], false, false, true, n_own, rows);
+  } else {
+    fill(p.part[0], false, s.Ls > 0, true, n_sh + n_own, rows);
+  }
+  if (p.part[1].splits == 0) p.part[1] = CtxPart{1, 0, 1, 0, 0, 0, 0};
+  if (p.slots > 1) p.bytes = (size_t)p.slots * s.B * s.Lq * s.H * (s.D + 2) * 4;
+  return p;
+}
+
+}  // namespace
+}  // namespace hb
+
+using namespace hb;
+
+extern "C" int hb_context_workspace_bytes(int batch, int q_len, int kv_len, int shared_len, int num_heads,
+                                          int kv_heads, int head_dim, size_t* bytes) {
+  if (!bytes) return HB_ERR_NULL;
+  const Shape s{batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim};
+  if (!shape_ok(s)) return HB_ERR_SHAPE;
+  *bytes = make_plan(s).bytes;
+  return HB_OK;
+}
+
+extern "C" int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, const void* kv,
+                               int64_t kv_batch_stride, int64_t kv_row_stride, const void* shared_kv,
+                               int64_t shared_row_stride, const int32_t* lens, const uint8_t* mask,
+                               int64_t mask_batch_stride, const uint8_t* shared_mask, const float* q_weight, float eps,
+                               float scale, void* out, int64_t out_batch_stride, int64_t out_row_stride, int batch,
+                               int q_len, int kv_len, int shared_len, int num_heads, int kv_heads, int head_dim,
+                               int dtype, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  if (!q || !out || (kv_len > 0 && !kv) || (shared_len > 0 && !shared_kv)) return HB_ERR_NULL;
+  const Shape s{batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim};
+  if (!shape_ok(s) || (dtype != HB_BF16 && dtype != HB_FP16)) return HB_ERR_SHAPE;
+  if (!(scale > 0.f) || !std::isfinite(scale) || (q_weight && !(eps >= 0.f))) return HB_ERR_SHAPE;
+  const int64_t qw = (int64_t)num_heads * head_dim, kw = 2ll * kv_heads * head_dim;
+  if (q_row_stride < qw || out_row_stride < qw || (kv_len > 1 && kv_row_stride < kw) ||
+      (shared_len > 1 && shared_row_stride < kw) || q_batch_stride < 0 || kv_batch_stride < 0 ||
+      (mask && mask_batch_stride < 0))
+    return HB_ERR_SHAPE;
+  // no two rows of the output share memory: batch elements one after the other, or interleaved row by row
+  if (batch > 1 && out_batch_stride < (q_len - 1) * out_row_stride + qw &&
+      (out_batch_stride < qw || out_row_stride < (batch - 1) * out_batch_stride + qw))
+    return HB_ERR_SHAPE;
+  const void* ptrs[] = {q, kv_len > 0 ? kv : nullptr, shared_len > 0 ? shared_kv : nullptr, out, workspace};
+  for (const void* pp : ptrs)
+    if (pp && !aligned16(pp)) return HB_ERR_ALIGN;
+  if (q_batch_stride % 8 || q_row_stride % 8 || kv_batch_stride % 8 || kv_row_stride % 8 || shared_row_stride % 8 ||
+      out_batch_stride % 8 || out_row_stride % 8)
+    return HB_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(lens) & 3u) || (reinterpret_cast<uintptr_t>(q_weight) & 15u)) return HB_ERR_ALIGN;
+  const Plan plan = make_plan(s);
+  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes)) return HB_ERR_WORKSPACE;
+  const int st = check_device();
+  if (st != HB_OK) return st;
+
+  CtxParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_bs = q_batch_stride;
+  p.q_rs = q_row_stride;
+  p.kv = static_cast<const uint16_t*>(kv);
+  p.kv_bs = kv_batch_stride;
+  p.kv_rs = kv_row_stride;
+  p.skv = static_cast<const uint16_t*>(shared_kv);
+  p.skv_rs = shared_row_stride;
+  p.lens = lens;
+  p.mask = mask;
+  p.mask_bs = mask_batch_stride;
+  p.smask = shared_mask;
+  p.q_w = q_weight;
+  p.eps = eps;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.out = static_cast<uint16_t*>(out);
+  p.o_bs = out_batch_stride;
+  p.o_rs = out_row_stride;
+  p.B = batch;
+  p.Lq = q_len;
+  p.H = num_heads;
+  p.Hkv = kv_heads;
+  p.G = num_heads / kv_heads;
+  p.Lkv = kv_len;
+  p.Ls = shared_len;
+  p.part[0] = plan.part[0];
+  p.part[1] = plan.part[1];
+  p.slots = plan.slots;
+  p.o_part = static_cast<float*>(workspace);
+  p.ml_part = plan.slots > 1 ? reinterpret_cast<float2*>(p.o_part + (size_t)plan.slots * batch * q_len * num_heads *
+                                                                        head_dim)
+                             : nullptr;
+  const bool fp16 = dtype == HB_FP16;
+  const int rc = launch_ctx_rows(p, head_dim, fp16, plan.rows_per_tile, stream);
+  if (rc != HB_OK || plan.slots == 1) return rc;
+  return launch_ctx_combine(p, head_dim, fp16, stream);
+}

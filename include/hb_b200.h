@@ -100,6 +100,44 @@ int hb_cross_diff_attn(const void* q, int64_t q_row_stride, const void* kv, int6
                        int64_t out_row_stride, int batch, int q_len, int kv_len, int num_heads, int head_dim,
                        float eps, cudaStream_t stream);
 
+/* ---- context attention (plain softmax over an encoder's states) ---------------------------------------- */
+/* Element types of the entry points that take more than bf16. */
+#define HB_BF16 0
+#define HB_FP16 1
+
+/* Bytes of workspace hb_context_attn needs for a call of these sizes: partial results of a key list that is cut
+ * over CTAs; 0 where it is not. */
+int hb_context_workspace_bytes(int batch, int q_len, int kv_len, int shared_len, int num_heads, int kv_heads,
+                               int head_dim, size_t* bytes);
+
+/* The attention of `sa3jax.dit._cross_attention` (dit.py:203-215) in its non-differential form (`_attend_out`'s
+ * plain `SDPA(q, k, v)`, dit.py:131-147), up to (not including) `to_out`, for contexts of any length, padded
+ * batches, fewer kv heads than query heads, and states that the whole batch shares:
+ *   out[b, i, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q[b, i, h] . k_j),
+ * j over the valid shared keys, then batch element b's valid own keys, of kv head h / (num_heads / kv_heads).
+ *   q         16-bit [batch, q_len, num_heads * head_dim] by strides (elements; batch stride >= 0).
+ *   kv        16-bit [batch, kv_len, k | v], kv_heads * head_dim columns each; may be NULL with kv_len 0.
+ *   shared_kv 16-bit [shared_len, k | v], the same for every batch element; may be NULL with shared_len 0.
+ *   lens      int32 [batch] or NULL: own keys j >= lens[b] are not read (clamped to [0, kv_len]).
+ *   mask      bytes [batch, kv_len] (row stride mask_batch_stride) or NULL: own keys with 0 are not read.
+ *   shared_mask  bytes [shared_len] or NULL.
+ *   q_weight  fp32 [head_dim] or NULL: each query head is RMS-normed first (dit.py:167-169: q * rsqrt(mean(q^2) +
+ *             eps) * q_weight, rounded to the 16-bit type as hb_head_rms_norm stores it).
+ *   out       16-bit [batch, q_len, num_heads * head_dim] by strides; must not overlap the inputs.
+ *   dtype     HB_BF16 or HB_FP16, for q, kv, shared_kv and out alike.
+ * A row without a valid key is written as zeros; what lies at keys that are not valid (infinities, NaN) does not
+ * reach the result. Scores, softmax statistics and sums are fp32; the weights p are rounded to the 16-bit type for
+ * the product with v (relative error at most 2^-8 or 2^-11 each), the sum of p is not. head_dim 64 or 128; rows of q, kv,
+ * shared_kv, out and their strides 16-byte aligned; scale > 0. The result does not depend on timing: the same call
+ * gives the same bits. Calls that may overlap on the GPU need workspaces of their own. */
+int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, const void* kv,
+                    int64_t kv_batch_stride, int64_t kv_row_stride, const void* shared_kv, int64_t shared_row_stride,
+                    const int32_t* lens, const uint8_t* mask, int64_t mask_batch_stride, const uint8_t* shared_mask,
+                    const float* q_weight, float eps, float scale, void* out, int64_t out_batch_stride,
+                    int64_t out_row_stride, int batch, int q_len, int kv_len, int shared_len, int num_heads,
+                    int kv_heads, int head_dim, int dtype, void* workspace, size_t workspace_bytes,
+                    cudaStream_t stream);
+
 /* ---- band (sliding-window) differential attention (SAME-L decoder) --------------------------------- */
 /* Bytes of workspace hb_band_diff_attn needs for `rows` buffer rows, `pair_count` head pairs, `window` and
  * rotate-half width `half`: a rows x half (cos, sin) table for window <= 128 (the fused kernel), prepared
