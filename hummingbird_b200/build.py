@@ -21,7 +21,7 @@ LIB = PKG / "libhb_b200.so"
 COMM_LIB = PKG / "libhb_comm.so"
 COMM_SOURCES = ["comm.cu"]
 SOURCES = ["abi.cu", "attn_kernel.cu", "attn_dense.cu", "dense_attn.cu", "band_attn.cu", "cross_attn.cu", "w8a8.cu",
-           "dit_glue.cu", "context_attn.cu", "context_rows.cu"]
+           "dit_glue.cu", "context_attn.cu", "context_rows.cu", "w4.cu"]
 # Compiled as whole-program device code (no -rdc) into an object linked into the same library: ptxas ignores
 # setmaxnreg in relocatable device code, and these kernels rebalance registers between warpgroups with it.
 WHOLE_PROGRAM_SOURCES = ["band_fused.cu", "band_proj.cu"]

@@ -1,0 +1,282 @@
+// Linear layers with 4-bit weights and group scales for a few rows (the conditioning vectors of a DiT step: one
+// row per clip), and the quantiser that lays their weights out.
+//
+//   y[m, n] = act(sum_k x[m, k] q[n, k] s[n, k / group] + bias[n]),  q in [-8, 7]
+//
+// With few rows the work is the bytes of the weights (1/2 + 2 / group per weight), so the layout makes them one
+// coalesced stream: blocks of 16 outputs x 128 inputs (1 KiB), in which a lane's two 16-byte loads are exactly its
+// share of the A operand of m16n8k16 MMAs (A: 16 outputs x 16 inputs, B: 16 inputs x 8 rows of x). Lane (row r, t)
+// holds inputs 32 w + 8 t .. + 8 of output rows r and r + 8 in its w-th words, so that 32 consecutive inputs are
+// one word step of the warp and every group of 32, 64 or 128 inputs ends at a step. The nibbles of a word are
+// ordered 0 2 4 6 1 3 5 7: shifting it by 4 i leaves inputs 2 i, 2 i + 1 in its two halves. A nibble u = q + 8 is
+// or-ed into the mantissa of 128 (bf16) or 1024 (fp16) and 136 or 1032 subtracted: q exactly, without a conversion.
+// Each group's sum is accumulated by the MMAs in fp32 and multiplied by its scale once, in fp32.
+//
+// One CTA takes 16 outputs; its eight warps take every eighth block of 128 inputs and merge through shared memory
+// in warp order, so the result does not depend on timing. x is read through L1 (it is the same few rows for
+// every CTA).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/hb_b200.h"
+#include "abi_common.h"
+#include "hb_sm100.cuh"
+#include "prep_common.cuh"
+
+namespace hb {
+namespace {
+
+constexpr int kWarps = 8;
+
+struct W4Params {
+  const uint16_t* x;
+  int64_t ldx;
+  const uint4* packed;
+  const uint16_t* scales;  // bf16 [tiles][blocks][128 / group][16]
+  const uint16_t* bias;
+  uint16_t* y;
+  int64_t ldy;
+  int M, N, K, kblocks, silu;
+};
+
+template <bool kFp16>
+struct Half;
+template <>
+struct Half<false> {
+  static __device__ __forceinline__ uint32_t weights(uint32_t w) {  // nibbles 0 and 4 of w
+    const uint32_t u = (w & 0x000f000fu) | 0x43004300u;
+    const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);
+    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), off);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ float load(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
+  static __device__ __forceinline__ uint16_t round(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+};
+template <>
+struct Half<true> {
+  static __device__ __forceinline__ uint32_t weights(uint32_t w) {
+    const uint32_t u = (w & 0x000f000fu) | 0x64006400u;
+    const __half2 off = __floats2half2_rn(1032.f, 1032.f);
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), off);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ float load(const uint16_t* p) { return __half2float(__ushort_as_half(*p)); }
+  static __device__ __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
+};
+
+template <bool kFp16, int NT, int kGroup>
+__global__ void __launch_bounds__(32 * kWarps) w4_linear_kernel(const W4Params p) {
+  using T = Half<kFp16>;
+  constexpr int kSteps = kGroup / 32;  // word steps per group
+  __shared__ float part[kWarps][16][8 * NT + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
+  const int tile = blockIdx.x, m0 = blockIdx.y * 8 * NT;
+
+  float acc[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+
+  const uint4* wp = p.packed + (int64_t)tile * p.kblocks * 64 + lane;
+  const uint16_t* sp = p.scales + (int64_t)tile * p.kblocks * (2048 / kGroup) + gid;
+  const uint16_t* xp[NT];
+  bool live[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int m = m0 + t * 8 + gid;
+    live[t] = m < p.M;
+    xp[t] = p.x + (live[t] ? m : 0) * p.ldx + tid * 8;
+  }
+
+  uint4 wa, wb;
+  int kb = warp;
+  if (kb < p.kblocks) {
+    wa = ld_nc_v4(wp + (int64_t)kb * 64);
+    wb = ld_nc_v4(wp + (int64_t)kb * 64 + 32);
+  }
+  while (kb < p.kblocks) {
+    const uint32_t lo[4] = {wa.x, wa.y, wa.z, wa.w}, hi[4] = {wb.x, wb.y, wb.z, wb.w};
+    const int k0 = kb * 128, next = kb + kWarps;
+    if (next < p.kblocks) {
+      wa = ld_nc_v4(wp + (int64_t)next * 64);
+      wb = ld_nc_v4(wp + (int64_t)next * 64 + 32);
+    }
+    float sc[128 / kGroup][2];
+#pragma unroll
+    for (int g = 0; g < 128 / kGroup; ++g) {
+      const uint16_t* s = sp + ((int64_t)kb * (128 / kGroup) + g) * 16;
+      sc[g][0] = __uint_as_float((uint32_t)__ldg(s) << 16);
+      sc[g][1] = __uint_as_float((uint32_t)__ldg(s + 8) << 16);
+    }
+    uint4 xv[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        xv[t][w] = live[t] && k0 + 32 * w < p.K ? __ldg(reinterpret_cast<const uint4*>(xp[t] + k0 + 32 * w))
+                                                : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int g = 0; g < 128 / kGroup; ++g) {
+      float c[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[t][e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int w = g * kSteps + s;
+        const uint32_t a0[4] = {T::weights(lo[w]), T::weights(hi[w]), T::weights(lo[w] >> 4), T::weights(hi[w] >> 4)};
+        const uint32_t a1[4] = {T::weights(lo[w] >> 8), T::weights(hi[w] >> 8), T::weights(lo[w] >> 12),
+                                T::weights(hi[w] >> 12)};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          T::mma(c[t], a0, xv[t][w].x, xv[t][w].y);
+          T::mma(c[t], a1, xv[t][w].z, xv[t][w].w);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(sc[g][e >> 1], c[t][e], acc[t][e]);
+    }
+    kb = next;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[warp][gid + 8 * (e >> 1)][t * 8 + tid * 2 + (e & 1)] = acc[t][e];
+  __syncthreads();
+  const int warps = min(kWarps, p.kblocks);
+  for (int i = threadIdx.x; i < 128 * NT; i += 32 * kWarps) {
+    const int r = i & 15, c = i >> 4, n = tile * 16 + r, m = m0 + c;
+    if (n >= p.N || m >= p.M) continue;
+    float v = part[0][r][c];
+    for (int w = 1; w < warps; ++w) v += part[w][r][c];
+    if (p.bias) v += T::load(p.bias + n);
+    if (p.silu) v = v / (1.f + expf(-v));
+    p.y[m * p.ldy + n] = T::round(v);
+  }
+}
+
+// Half a warp per (output row, 128-input block): lane i holds inputs 8 i .. 8 i + 8. Rows past N and inputs past K
+// become zeros with scale 0, so the linear layer reads whole blocks.
+template <int kGroup>
+__global__ void __launch_bounds__(256) w4_quant_kernel(const uint16_t* __restrict__ w, int64_t ldw, int N, int K,
+                                                       int tiles, int kblocks, uint32_t* __restrict__ packed,
+                                                       uint16_t* __restrict__ scales) {
+  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
+  const int i = threadIdx.x & 15;
+  if (unit >= (int64_t)tiles * 16 * kblocks) return;  // whole half-warps; the shuffles below stay inside one
+  const int64_t row = unit / kblocks;
+  const int kb = static_cast<int>(unit - row * kblocks);
+  const int k = kb * 128 + i * 8;
+  const bool live = row < N && k < K;
+  float v[8];
+  if (live) {
+    unpack8(__ldg(reinterpret_cast<const uint4*>(w + row * ldw + k)), v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  }
+  float amax = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
+  const unsigned half = 0xffffu << (threadIdx.x & 16);
+#pragma unroll
+  for (int o = 1; o < kGroup / 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(half, amax, o));
+  float s = bf16_lo(__bfloat16_as_ushort(__float2bfloat16_rn(__fdiv_rn(amax, 7.f))));
+  if (s == 0.f) s = 1.f;
+  uint32_t word = 0u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int q = static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(v[e], s)), -7.f), 7.f)) + 8;
+    word |= static_cast<uint32_t>(q) << (4 * ((e >> 1) + 4 * (e & 1)));
+  }
+  const int64_t tile = row >> 4;
+  const int r = static_cast<int>(row & 15), t = i & 3, ws = i >> 2;
+  packed[(tile * kblocks + kb) * 256 + (r >> 3) * 128 + (r & 7) * 16 + t * 4 + ws] = word;
+  if (i % (kGroup / 8) == 0)
+    scales[((tile * kblocks + kb) * (128 / kGroup) + i / (kGroup / 8)) * 16 + r] =
+        live ? __bfloat16_as_ushort(__float2bfloat16_rn(s)) : 0;
+}
+
+template <bool kFp16, int NT>
+void launch_linear(const W4Params& p, int group, dim3 grid, cudaStream_t s) {
+  if (group == 32) w4_linear_kernel<kFp16, NT, 32><<<grid, 32 * kWarps, 0, s>>>(p);
+  if (group == 64) w4_linear_kernel<kFp16, NT, 64><<<grid, 32 * kWarps, 0, s>>>(p);
+  if (group == 128) w4_linear_kernel<kFp16, NT, 128><<<grid, 32 * kWarps, 0, s>>>(p);
+}
+template <bool kFp16>
+void launch_linear(const W4Params& p, int nt, int group, dim3 grid, cudaStream_t s) {
+  if (nt == 1) launch_linear<kFp16, 1>(p, group, grid, s);
+  if (nt == 2) launch_linear<kFp16, 2>(p, group, grid, s);
+  if (nt == 4) launch_linear<kFp16, 4>(p, group, grid, s);
+}
+
+bool w4_shape_ok(int N, int K, int group) {
+  return N >= 1 && K >= 1 && (group == 32 || group == 64 || group == 128) && K % group == 0 && N < (1 << 30) &&
+         K < (1 << 30);
+}
+
+}  // namespace
+}  // namespace hb
+
+using namespace hb;
+
+extern "C" int hb_quant_w4(const void* w, int64_t ldw, int N, int K, int group, void* packed, void* scales,
+                           cudaStream_t stream) {
+  if (!w || !packed || !scales) return HB_ERR_NULL;
+  if (!w4_shape_ok(N, K, group) || ldw < K) return HB_ERR_SHAPE;
+  if (!aligned16(w) || !aligned16(packed) || !aligned16(scales) || ldw % 8) return HB_ERR_ALIGN;
+  const int st = check_device();
+  if (st != HB_OK) return st;
+  const int tiles = (N + 15) / 16, kblocks = (K + 127) / 128;
+  const int64_t grid = ((int64_t)tiles * 16 * kblocks * 16 + 255) / 256;
+  if (grid >= (1ll << 31)) return HB_ERR_SHAPE;
+  const uint16_t* wp = static_cast<const uint16_t*>(w);
+  uint32_t* pp = static_cast<uint32_t*>(packed);
+  uint16_t* sp = static_cast<uint16_t*>(scales);
+  const unsigned g = static_cast<unsigned>(grid);
+  if (group == 32) w4_quant_kernel<32><<<g, 256, 0, stream>>>(wp, ldw, N, K, tiles, kblocks, pp, sp);
+  if (group == 64) w4_quant_kernel<64><<<g, 256, 0, stream>>>(wp, ldw, N, K, tiles, kblocks, pp, sp);
+  if (group == 128) w4_quant_kernel<128><<<g, 256, 0, stream>>>(wp, ldw, N, K, tiles, kblocks, pp, sp);
+  return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
+}
+
+extern "C" int hb_w4_linear(const void* x, int64_t ldx, const void* packed, const void* scales, const void* bias,
+                            void* y, int64_t ldy, int M, int N, int K, int group, int silu, int dtype,
+                            cudaStream_t stream) {
+  if (!x || !packed || !scales || !y) return HB_ERR_NULL;
+  if (!w4_shape_ok(N, K, group) || M < 1 || M > 32 * 65535 || ldx < K || ldy < N ||
+      (dtype != HB_BF16 && dtype != HB_FP16) || (silu != 0 && silu != 1))
+    return HB_ERR_SHAPE;
+  if (!aligned16(x) || !aligned16(packed) || !aligned16(scales) || ldx % 8 || (reinterpret_cast<uintptr_t>(y) & 1u) ||
+      (reinterpret_cast<uintptr_t>(bias) & 1u))
+    return HB_ERR_ALIGN;
+  const int st = check_device();
+  if (st != HB_OK) return st;
+  const W4Params p{static_cast<const uint16_t*>(x), ldx, static_cast<const uint4*>(packed),
+                   static_cast<const uint16_t*>(scales), static_cast<const uint16_t*>(bias),
+                   static_cast<uint16_t*>(y), ldy, M, N, K, (K + 127) / 128, silu};
+  const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4;
+  const dim3 grid((N + 15) / 16, (M + 8 * nt - 1) / (8 * nt));
+  if (dtype == HB_FP16)
+    launch_linear<true>(p, nt, group, grid, stream);
+  else
+    launch_linear<false>(p, nt, group, grid, stream);
+  return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
+}

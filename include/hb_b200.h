@@ -226,6 +226,28 @@ int hb_w8a8_gemm(const void* qx, int64_t ldqx, const float* sx, const void* qw, 
 int hb_w8a8_gemm_glu(const void* qx, int64_t ldqx, const float* sx, const void* qw, int64_t ldqw, const float* sw,
                      const void* bias, void* z, int64_t ldz, int M, int F, int K, cudaStream_t stream);
 
+/* ---- W4 linear layers for a few rows (the DiT's conditioning vectors) -------------------------------------- */
+/* 4-bit weights with a scale per output row and group of 32, 64 or 128 inputs, from a bf16 matrix w [N, K] (leading
+ * dim ldw elements): s = bf16(absmax / 7) of the group (1 where that is 0), q = clamp(rint(w / s), -7, 7) with the
+ * correctly rounded fp32 quotient, ties to even. K a multiple of group; w finite.
+ *   packed  1,024 bytes per block of 16 rows x 128 inputs, blocks [ceil(N / 16)][ceil(K / 128)]: the 32-bit word at
+ *           byte 512 * (r / 8) + 64 * (r % 8) + 16 * t + 4 * u holds row r's inputs 32 u + 8 t .. + 8 of the block;
+ *           its nibbles, lowest first, are those inputs 0, 2, 4, 6, 1, 3, 5, 7, each q + 8. Rows past N and inputs
+ *           past K hold 8 (zero).
+ *   scales  bf16 [ceil(N / 16)][ceil(K / 128)][128 / group][16 rows]; 0 past N and K.
+ * No reference counterpart: the reference's conditioning embedders are bf16 `_linear`s (dit.py:33-42). */
+int hb_quant_w4(const void* w, int64_t ldw, int N, int K, int group, void* packed, void* scales, cudaStream_t stream);
+
+/* y[m, n] = act(sum_k x[m, k] * q[n, k] * s[n, k / group] + bias[n]) for weights of hb_quant_w4's layout (any q in
+ * [-8, 7]); replaces `dit._linear` (dit.py:33-36) where few rows go through it, as in the timestep, global and adaLN
+ * embedders (dit.py:39-42), whose SiLU can be taken along.
+ *   x [M, K] (ldx elements, rows 16-byte aligned), bias [N] or NULL, y [M, N] (ldy elements): bf16 or fp16 (dtype).
+ *   silu  1: act(v) = v / (1 + exp(-v)); 0: none.
+ * fp32 sums, one rounding at the end; the same call gives the same bits. Any M is computed; the weights are read once
+ * for every 32 rows, so beyond a few dozen rows a W8A8 GEMM is the faster layer. */
+int hb_w4_linear(const void* x, int64_t ldx, const void* packed, const void* scales, const void* bias, void* y,
+                 int64_t ldy, int M, int N, int K, int group, int silu, int dtype, cudaStream_t stream);
+
 /* ---- DiT block glue (the elementwise steps around the kernels above) ------------------------------------ */
 /* No reference counterpart as entry points: the reference runs these steps as separate XLA ops inside
  * `dit._block` (dit.py:224-250); here each fuses several of them into one pass over the activation rows.
