@@ -42,10 +42,14 @@ def _rows(t: torch.Tensor, name: str, width: int, dtype: torch.dtype, device: to
 
 
 def _readable(t: torch.Tensor, width: int) -> torch.Tensor:
+    """`t`, or a copy of it where a tensor map cannot describe its rows."""
     strides = t.stride()
-    if strides[-1] == 1 and t.data_ptr() % 16 == 0 and strides[-2] >= width \
-            and not any(s % 8 or s < 0 for s in strides[:-1]):
-        return t
+    if strides[-1] == 1 and t.data_ptr() % 16 == 0 and strides[-2] >= width and strides[-2] % 8 == 0:
+        if t.dim() == 2:
+            return t
+        row, batch = strides[1], strides[0]
+        if batch == 0 or (batch >= width and batch % 8 == 0 and (batch % row == 0 or row % batch == 0)):
+            return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
 
@@ -96,7 +100,8 @@ def _attend(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_
         out = torch.empty(batch, q_len, width, dtype=dtype, device=device)
     if not batch or not q_len:
         return out
-    need = _workspace_bytes(batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim)
+    need = _workspace_bytes(batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim,
+                            int(mask is not None or shared_mask is not None))
     # partial results in a block of the caching allocator: it belongs to this call's stream, or to the graph that
     # is being captured, so calls on other streams and other graphs have theirs
     with torch.cuda.device(device):

@@ -10,63 +10,70 @@
 namespace hb {
 namespace {
 
-constexpr int kSms = 148;
-constexpr int kMaxSlots = 256;
+constexpr int kCtas = 2 * 148;         // CTAs that run at once: two per SM, of either kernel
+constexpr int kMaxSplits = 128;        // of a part, where nothing forces more
+constexpr int kMaxKeys = 1 << 24;
+constexpr int kRowsKernelMax = 32;     // rows of an item up to which it goes to the few-rows kernel
 
 struct Shape {
-  int B, Lq, Lkv, Ls, H, Hkv, D;
+  int B, Lq, Lkv, Ls, H, Hkv, D, masked;
 };
 
 struct Plan {
   CtxPart part[2];
+  bool tiles[2];       // the part runs on the tcgen05 kernel
+  int rows_per_tile;   // of the few-rows kernel
+  int mask_tiles;      // most key tiles of a CTA of the tcgen05 kernel
   int slots;
-  int rows_per_tile;
-  size_t bytes;  // partial results
+  size_t bytes;        // partial results
 };
 
 bool shape_ok(const Shape& s) {
   if (s.B < 1 || s.Lq < 1 || s.Lkv < 0 || s.Ls < 0 || s.H < 1 || s.Hkv < 1 || s.H % s.Hkv) return false;
-  if (s.D != 64 && s.D != 128) return false;
+  if ((s.D != 64 && s.D != 128) || (s.masked != 0 && s.masked != 1)) return false;
   // a kv head's rows over the whole batch, and the items of a call, are counted in 32 bits
-  const int64_t rows = (int64_t)s.B * s.Lq * s.H;
-  return rows < (1ll << 30) && s.Lkv < (1 << 30) && s.Ls < (1 << 30);
+  return s.Lkv <= kMaxKeys && s.Ls <= kMaxKeys && s.H < (1 << 16) && s.B <= (1 << 28) / s.H &&
+         (int64_t)s.B * s.Lq * s.H < (1ll << 28);
 }
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
-// Parts of a list of `chunks` key chunks over `items` items: two CTAs for every SM where the list is long enough
-// to give each of a CTA's four warps two chunks.
-int splits_for(int64_t items, int chunks) {
-  const int want = ceil_div(2 * kSms, items);
-  return std::max(1, std::min(want, std::max(1, chunks / 8)));
-}
-
 Plan make_plan(const Shape& s) {
   Plan p{};
-  const int G = s.H / s.Hkv, kc = 2048 / s.D;
+  const int G = s.H / s.Hkv;
   const int rows = s.Lq * G;
+  // One pass over the shared keys for all batch elements pays where an element's rows would leave most of a
+  // 128-row tile empty; otherwise each element walks them in the same pass as its own.
   const bool pooled = s.Ls > 0 && s.B > 1 && rows < 128;
-  const int rows0 = pooled ? rows * s.B : rows;
-  p.rows_per_tile = s.D == 64 && rows0 > 16 ? 32 : 16;
-  const int n_sh = ceil_div(s.Ls, kc), n_own = ceil_div(s.Lkv, kc);
-  auto fill = [&](CtxPart& part, bool pool, bool sh, bool own, int chunks, int part_rows) {
+  auto fill = [&](int i, bool pool, bool sh, bool own, int part_rows) {
+    CtxPart& part = p.part[i];
+    const bool tiles = p.tiles[i] = part_rows > kRowsKernelMax;
     part.pooled = pool;
     part.use_shared = sh;
     part.use_own = own;
-    part.row_tiles = ceil_div(part_rows, p.rows_per_tile);
+    const int tile_rows = tiles ? 128 : p.rows_per_tile;
+    part.row_tiles = ceil_div(part_rows, tile_rows);
     const int64_t items = (int64_t)(pool ? 1 : s.B) * s.Hkv * part.row_tiles;
-    part.splits = std::min(splits_for(items, chunks), kMaxSlots / 2);
+    const int keys = tiles ? 128 : 2048 / s.D;
+    const int chunks = (sh ? ceil_div(s.Ls, keys) : 0) + (own ? ceil_div(s.Lkv, keys) : 0);
+    // Few items: the key list is cut so that one round of CTAs fills the GPU, down to two tiles (or two chunks for
+    // each of the four warps) per CTA; the merge then costs less than the idle SMs.
+    part.splits = std::max(1, std::min({static_cast<int>(kCtas / items), chunks / (tiles ? 2 : 8), kMaxSplits}));
+    if (tiles && s.masked) part.splits = std::max(part.splits, ceil_div(chunks, kCtxMaskTiles));
+    if (tiles && s.masked) p.mask_tiles = std::max(p.mask_tiles, ceil_div(chunks, part.splits));
     part.slot0 = p.slots;
     part.ctas = static_cast<int>(items * part.splits);
     p.slots += part.splits;
   };
+  const int rows0 = pooled ? rows * s.B : rows;
+  p.rows_per_tile = s.D == 64 && (rows0 <= kRowsKernelMax ? rows0 : rows) > 16 ? 32 : 16;
+  p.part[1] = CtxPart{1, 0, 1, 0, 0, 0, 0};
   if (pooled) {
-    fill(p.part[0], true, true, false, n_sh, rows0);
-    if (s.Lkv > 0) fill(p.part[1], false, false, true, n_own, rows);
+    fill(0, true, true, false, rows0);
+    if (s.Lkv > 0) fill(1, false, false, true, rows);
   } else {
-    fill(p.part[0], false, s.Ls > 0, true, n_sh + n_own, rows);
+    fill(0, false, s.Ls > 0, true, rows);
   }
-  if (p.part[1].splits == 0) p.part[1] = CtxPart{1, 0, 1, 0, 0, 0, 0};
   if (p.slots > 1) p.bytes = (size_t)p.slots * s.B * s.Lq * s.H * (s.D + 2) * 4;
   return p;
 }
@@ -77,9 +84,9 @@ Plan make_plan(const Shape& s) {
 using namespace hb;
 
 extern "C" int hb_context_workspace_bytes(int batch, int q_len, int kv_len, int shared_len, int num_heads,
-                                          int kv_heads, int head_dim, size_t* bytes) {
+                                          int kv_heads, int head_dim, int masked, size_t* bytes) {
   if (!bytes) return HB_ERR_NULL;
-  const Shape s{batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim};
+  const Shape s{batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim, masked};
   if (!shape_ok(s)) return HB_ERR_SHAPE;
   *bytes = make_plan(s).bytes;
   return HB_OK;
@@ -93,7 +100,7 @@ extern "C" int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_
                                int q_len, int kv_len, int shared_len, int num_heads, int kv_heads, int head_dim,
                                int dtype, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   if (!q || !out || (kv_len > 0 && !kv) || (shared_len > 0 && !shared_kv)) return HB_ERR_NULL;
-  const Shape s{batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim};
+  const Shape s{batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim, mask || shared_mask ? 1 : 0};
   if (!shape_ok(s) || (dtype != HB_BF16 && dtype != HB_FP16)) return HB_ERR_SHAPE;
   if (!(scale > 0.f) || !std::isfinite(scale) || (q_weight && !(eps >= 0.f))) return HB_ERR_SHAPE;
   const int64_t qw = (int64_t)num_heads * head_dim, kw = 2ll * kv_heads * head_dim;
@@ -101,6 +108,8 @@ extern "C" int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_
       (shared_len > 1 && shared_row_stride < kw) || q_batch_stride < 0 || kv_batch_stride < 0 ||
       (mask && mask_batch_stride < 0))
     return HB_ERR_SHAPE;
+  constexpr int64_t kMaxStride = (1ll << 39) - 1;  // a tensor map's: below 2^40 bytes
+  if (kv_batch_stride > kMaxStride || kv_row_stride > kMaxStride || shared_row_stride > kMaxStride) return HB_ERR_SHAPE;
   // no two rows of the output share memory: batch elements one after the other, or interleaved row by row
   if (batch > 1 && out_batch_stride < (q_len - 1) * out_row_stride + qw &&
       (out_batch_stride < qw || out_row_stride < (batch - 1) * out_batch_stride + qw))
@@ -112,6 +121,13 @@ extern "C" int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_
       out_batch_stride % 8 || out_row_stride % 8)
     return HB_ERR_ALIGN;
   if ((reinterpret_cast<uintptr_t>(lens) & 3u) || (reinterpret_cast<uintptr_t>(q_weight) & 15u)) return HB_ERR_ALIGN;
+  // What a tensor map describes: rows of at least their width; batch elements one after the other or interleaved
+  // row by row, the larger stride a multiple of the smaller (or all of them the same rows: stride 0).
+  const bool inter = batch > 1 && kv_len > 1 && kv_batch_stride > 0 && kv_batch_stride < kv_row_stride;
+  if (batch > 1 && kv_len > 0 && kv_batch_stride > 0) {
+    if (kv_batch_stride < kw) return HB_ERR_SHAPE;
+    if (kv_len > 1 && (inter ? kv_row_stride % kv_batch_stride : kv_batch_stride % kv_row_stride)) return HB_ERR_ALIGN;
+  }
   const Plan plan = make_plan(s);
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes)) return HB_ERR_WORKSPACE;
   const int st = check_device();
@@ -123,9 +139,11 @@ extern "C" int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_
   p.q_rs = q_row_stride;
   p.kv = static_cast<const uint16_t*>(kv);
   p.kv_bs = kv_batch_stride;
-  p.kv_rs = kv_row_stride;
+  p.kv_rs = kv_len > 1 ? kv_row_stride : std::max(kv_row_stride, kw);
+  if (kv_len == 1 && batch > 1 && kv_batch_stride > 0) p.kv_rs = kv_batch_stride;
+  p.kv_inter = inter;
   p.skv = static_cast<const uint16_t*>(shared_kv);
-  p.skv_rs = shared_row_stride;
+  p.skv_rs = shared_len > 1 ? shared_row_stride : std::max(shared_row_stride, kw);
   p.lens = lens;
   p.mask = mask;
   p.mask_bs = mask_batch_stride;
@@ -143,15 +161,21 @@ extern "C" int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_
   p.G = num_heads / kv_heads;
   p.Lkv = kv_len;
   p.Ls = shared_len;
-  p.part[0] = plan.part[0];
-  p.part[1] = plan.part[1];
   p.slots = plan.slots;
   p.o_part = static_cast<float*>(workspace);
   p.ml_part = plan.slots > 1 ? reinterpret_cast<float2*>(p.o_part + (size_t)plan.slots * batch * q_len * num_heads *
                                                                         head_dim)
                              : nullptr;
   const bool fp16 = dtype == HB_FP16;
-  const int rc = launch_ctx_rows(p, head_dim, fp16, plan.rows_per_tile, stream);
-  if (rc != HB_OK || plan.slots == 1) return rc;
-  return launch_ctx_combine(p, head_dim, fp16, stream);
+  for (int kernel = 0; kernel < 2; ++kernel) {  // the parts of the few-rows kernel, then those of the tcgen05 one
+    for (int i = 0; i < 2; ++i) {
+      p.part[i] = plan.part[i];
+      if (plan.tiles[i] != (kernel == 1)) p.part[i].ctas = 0;
+    }
+    if (p.part[0].ctas + p.part[1].ctas == 0) continue;
+    const int rc = kernel ? launch_ctx_tiles(p, head_dim, fp16, plan.mask_tiles, stream)
+                          : launch_ctx_rows(p, head_dim, fp16, plan.rows_per_tile, stream);
+    if (rc != HB_OK) return rc;
+  }
+  return plan.slots > 1 ? launch_ctx_combine(p, head_dim, fp16, stream) : HB_OK;
 }

@@ -24,6 +24,7 @@ struct CtxParams {
   int64_t q_bs, q_rs;
   const uint16_t* kv;     // [batch, kv_len, k | v], kv_heads * D each
   int64_t kv_bs, kv_rs;
+  int kv_inter;           // batch elements interleaved row by row (kv_bs < kv_rs)
   const uint16_t* skv;    // [shared_len, k | v]
   int64_t skv_rs;
   const int32_t* lens;    // [batch] or null: keys at and past lens[b] are not read
@@ -47,9 +48,18 @@ __device__ __forceinline__ int ctx_own_len(const CtxParams& p, int b) {
   return p.lens ? max(0, min(p.lens[b], p.Lkv)) : p.Lkv;
 }
 
-// Launchers: a CUDA error (or a kernel that cannot be launched) returns HB_ERR_LAUNCH.
-// The few-rows kernel (context_rows.cu); rows_per_tile 16, or 32 at D 64.
+// Mask bits of a CTA's keys are kept in its shared memory, 16 bytes per 128 keys, for at most this many tiles.
+constexpr int kCtxMaskTiles = 512;
+
+// Launchers of the parts whose `ctas` is not 0: a CUDA error (or a kernel that cannot be launched) returns
+// HB_ERR_LAUNCH. The few-rows kernel (context_rows.cu; rows_per_tile 16, or 32 at D 64), the tcgen05 kernel on
+// 128-row tiles (context_tiles.cu; `mask_tiles`: the most key tiles of a CTA where there is a mask), and the merge
+// of partial results (context_rows.cu).
 int launch_ctx_rows(const CtxParams& p, int D, bool fp16, int rows_per_tile, cudaStream_t stream);
+int launch_ctx_tiles(const CtxParams& p, int D, bool fp16, int mask_tiles, cudaStream_t stream);
 int launch_ctx_combine(const CtxParams& p, int D, bool fp16, cudaStream_t stream);
+
+// Read (and clear, when set) the status word of the tcgen05 kernel's translation unit on the current device.
+int ctx_tiles_take_status(unsigned int* status);
 
 }  // namespace hb

@@ -106,9 +106,9 @@ int hb_cross_diff_attn(const void* q, int64_t q_row_stride, const void* kv, int6
 #define HB_FP16 1
 
 /* Bytes of workspace hb_context_attn needs for a call of these sizes: partial results of a key list that is cut
- * over CTAs; 0 where it is not. */
+ * over CTAs; 0 where it is not. masked: 1 if the call has a mask or a shared mask, else 0. */
 int hb_context_workspace_bytes(int batch, int q_len, int kv_len, int shared_len, int num_heads, int kv_heads,
-                               int head_dim, size_t* bytes);
+                               int head_dim, int masked, size_t* bytes);
 
 /* The attention of `sa3jax.dit._cross_attention` (dit.py:203-215) in its non-differential form (`_attend_out`'s
  * plain `SDPA(q, k, v)`, dit.py:131-147), up to (not including) `to_out`, for contexts of any length, padded
@@ -128,7 +128,8 @@ int hb_context_workspace_bytes(int batch, int q_len, int kv_len, int shared_len,
  * A row without a valid key is written as zeros; what lies at keys that are not valid (infinities, NaN) does not
  * reach the result. Scores, softmax statistics and sums are fp32; the weights p are rounded to the 16-bit type for
  * the product with v (relative error at most 2^-8 or 2^-11 each), the sum of p is not. head_dim 64 or 128; rows of q, kv,
- * shared_kv, out and their strides 16-byte aligned; scale > 0. The result does not depend on timing: the same call
+ * shared_kv, out and their strides 16-byte aligned; kv's batch stride 0, or one of its two strides a multiple of the
+ * other; kv_len and shared_len at most 2^24; scale > 0. The result does not depend on timing: the same call
  * gives the same bits. Calls that may overlap on the GPU need workspaces of their own. */
 int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, const void* kv,
                     int64_t kv_batch_stride, int64_t kv_row_stride, const void* shared_kv, int64_t shared_row_stride,

@@ -17,9 +17,9 @@ def lib():
     return _lib.lib()
 
 
-def _need(lib, *sizes):
+def _need(lib, *sizes, masked=0):
     n = ctypes.c_size_t(0)
-    assert lib.hb_context_workspace_bytes(*sizes, ctypes.byref(n)) == _lib.HB_OK
+    assert lib.hb_context_workspace_bytes(*sizes, masked, ctypes.byref(n)) == _lib.HB_OK
     return n.value
 
 
@@ -56,6 +56,11 @@ def _args(**kw):
     (dict(o_bs=1024), _lib.HB_ERR_SHAPE),                      # output rows of two batch elements on one another
     (dict(q_bs=-1024), _lib.HB_ERR_SHAPE),
     (dict(batch=1 << 20, q_len=1 << 20), _lib.HB_ERR_SHAPE),
+    (dict(kv_len=(1 << 24) + 1), _lib.HB_ERR_SHAPE),
+    (dict(kv_bs=1024), _lib.HB_ERR_SHAPE),                     # batch elements closer than a row
+    (dict(kv_bs=257 * 2048 + 8), _lib.HB_ERR_ALIGN),           # neither stride a multiple of the other
+    (dict(kv_bs=2056, kv_rs=4096), _lib.HB_ERR_ALIGN),
+    (dict(kv_rs=1 << 40), _lib.HB_ERR_SHAPE),
     (dict(q=P + 8), _lib.HB_ERR_ALIGN),
     (dict(kv=P + 2), _lib.HB_ERR_ALIGN),
     (dict(out=P + 4), _lib.HB_ERR_ALIGN),
@@ -77,8 +82,8 @@ def test_workspace_is_asked_for_and_checked(lib):
     assert lib.hb_context_attn(*_args(**one, ws_bytes=need - 1)) == _lib.HB_ERR_WORKSPACE
     assert _need(lib, 1, 1, 16, 0, 16, 16, 64) == 0             # one part: written directly
     n = ctypes.c_size_t(0)
-    assert lib.hb_context_workspace_bytes(1, 1, 16, 0, 16, 5, 64, ctypes.byref(n)) == _lib.HB_ERR_SHAPE
-    assert lib.hb_context_workspace_bytes(1, 1, 16, 0, 16, 16, 64, None) == _lib.HB_ERR_NULL
+    assert lib.hb_context_workspace_bytes(1, 1, 16, 0, 16, 5, 64, 0, ctypes.byref(n)) == _lib.HB_ERR_SHAPE
+    assert lib.hb_context_workspace_bytes(1, 1, 16, 0, 16, 16, 64, 0, None) == _lib.HB_ERR_NULL
 
 
 def test_workspace_stays_small_against_the_inputs(lib):
