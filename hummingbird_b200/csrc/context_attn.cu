@@ -10,7 +10,6 @@
 namespace hb {
 namespace {
 
-constexpr int kCtas = 2 * 148;         // CTAs that run at once: two per SM, of either kernel
 constexpr int kMaxSplits = 128;        // of a part, where nothing forces more
 constexpr int kMaxKeys = 1 << 24;
 constexpr int kRowsKernelMax = 32;     // rows of an item up to which it goes to the few-rows kernel
@@ -23,8 +22,8 @@ struct Plan {
   CtxPart part[2];
   bool tiles[2];       // the part runs on the tcgen05 kernel
   int rows_per_tile;   // of the few-rows kernel
-  int mask_tiles;      // most key tiles of a CTA of the tcgen05 kernel
-  int slots;
+  int mask_tiles;      // most key tiles of a unit of the tcgen05 kernel
+  int slots, prows, tail_rows;
   size_t bytes;        // partial results
 };
 
@@ -38,6 +37,22 @@ bool shape_ok(const Shape& s) {
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
+// Into how many parts the key lists (n tiles each) of the units that a last, partly filled round of CTAs would take
+// are cut: the parts' rounds, at 1.5 tiles of fixed cost a unit, and for any cut the merge, about 5 tiles' time
+// (a tile: 0.8 us).
+int tail_splits(int units, int n) {
+  int best = 1;
+  double best_cost = n + 1.5;
+  for (int k = 2; k <= 16 && n / k >= 4; ++k) {
+    const double cost = ceil_div((int64_t)units * k, kCtxRound) * (ceil_div(n, k) + 1.5) + 5;
+    if (cost < best_cost) {
+      best = k;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
 Plan make_plan(const Shape& s) {
   Plan p{};
   const int G = s.H / s.Hkv;
@@ -45,36 +60,57 @@ Plan make_plan(const Shape& s) {
   // One pass over the shared keys for all batch elements pays where an element's rows would leave most of a
   // 128-row tile empty; otherwise each element walks them in the same pass as its own.
   const bool pooled = s.Ls > 0 && s.B > 1 && rows < 128;
+  const int rows0 = pooled ? rows * s.B : rows;
+  p.rows_per_tile = s.D == 64 && (rows0 <= kRowsKernelMax ? rows0 : rows) > 16 ? 32 : 16;
   auto fill = [&](int i, bool pool, bool sh, bool own, int part_rows) {
     CtxPart& part = p.part[i];
     const bool tiles = p.tiles[i] = part_rows > kRowsKernelMax;
     part.pooled = pool;
     part.use_shared = sh;
     part.use_own = own;
-    const int tile_rows = tiles ? 128 : p.rows_per_tile;
-    part.row_tiles = ceil_div(part_rows, tile_rows);
+    part.row_tiles = ceil_div(part_rows, tiles ? 128 : p.rows_per_tile);
     const int64_t items = (int64_t)(pool ? 1 : s.B) * s.Hkv * part.row_tiles;
     const int keys = tiles ? 128 : 2048 / s.D;
     const int chunks = (sh ? ceil_div(s.Ls, keys) : 0) + (own ? ceil_div(s.Lkv, keys) : 0);
     // Few items: the key list is cut so that one round of CTAs fills the GPU, down to two tiles (or two chunks for
     // each of the four warps) per CTA; the merge then costs less than the idle SMs.
-    part.splits = std::max(1, std::min({static_cast<int>(kCtas / items), chunks / (tiles ? 2 : 8), kMaxSplits}));
+    part.splits = std::max(1, std::min({static_cast<int>(kCtxRound / items), chunks / (tiles ? 2 : 8), kMaxSplits}));
     if (tiles && s.masked) part.splits = std::max(part.splits, ceil_div(chunks, kCtxMaskTiles));
-    if (tiles && s.masked) p.mask_tiles = std::max(p.mask_tiles, ceil_div(chunks, part.splits));
+    part.count = static_cast<int>(items * part.splits);
     part.slot0 = p.slots;
-    part.ctas = static_cast<int>(items * part.splits);
     p.slots += part.splits;
+    if (tiles && !pooled && part.splits == 1 && items > kCtxRound && items % kCtxRound) {
+      // Many items, and a last round that leaves CTAs idle: its items alone are cut.
+      const int tail = static_cast<int>(items % kCtxRound), k = tail_splits(tail, chunks);
+      if (k > 1) {
+        CtxPart& last = p.part[1] = part;
+        part.count = static_cast<int>(items - tail);
+        last.item0 = part.count;
+        last.splits = k;
+        last.count = tail * k;
+        p.tiles[1] = true;
+        p.tail_rows = 128;
+        p.slots = k;
+      }
+    }
+    if (tiles && s.masked) p.mask_tiles = std::max(p.mask_tiles, ceil_div(chunks, part.splits));
   };
-  const int rows0 = pooled ? rows * s.B : rows;
-  p.rows_per_tile = s.D == 64 && (rows0 <= kRowsKernelMax ? rows0 : rows) > 16 ? 32 : 16;
-  p.part[1] = CtxPart{1, 0, 1, 0, 0, 0, 0};
   if (pooled) {
     fill(0, true, true, false, rows0);
     if (s.Lkv > 0) fill(1, false, false, true, rows);
   } else {
     fill(0, false, s.Ls > 0, true, rows);
   }
-  if (p.slots > 1) p.bytes = (size_t)p.slots * s.B * s.Lq * s.H * (s.D + 2) * 4;
+  for (CtxPart& part : p.part) {
+    if (part.count == 0) part.splits = part.row_tiles = 1;
+    part.by_splits = fast_div(part.splits);
+    part.by_row_tiles = fast_div(part.row_tiles);
+    part.direct = p.slots == 1 || (p.tail_rows && &part == &p.part[0]);
+  }
+  if (p.slots > 1) {
+    p.prows = p.tail_rows ? p.part[1].count / p.part[1].splits * p.tail_rows : s.B * s.Lq * s.H;
+    p.bytes = (size_t)p.slots * p.prows * (s.D + 2) * 4;
+  }
   return p;
 }
 
@@ -117,6 +153,7 @@ extern "C" int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_
   const void* ptrs[] = {q, kv_len > 0 ? kv : nullptr, shared_len > 0 ? shared_kv : nullptr, out, workspace};
   for (const void* pp : ptrs)
     if (pp && !aligned16(pp)) return HB_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(workspace) % 32) return HB_ERR_ALIGN;
   if (q_batch_stride % 8 || q_row_stride % 8 || kv_batch_stride % 8 || kv_row_stride % 8 || shared_row_stride % 8 ||
       out_batch_stride % 8 || out_row_stride % 8)
     return HB_ERR_ALIGN;
@@ -154,6 +191,7 @@ extern "C" int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_
   p.out = static_cast<uint16_t*>(out);
   p.o_bs = out_batch_stride;
   p.o_rs = out_row_stride;
+  p.out_wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && out_row_stride % 16 == 0 && out_batch_stride % 16 == 0;
   p.B = batch;
   p.Lq = q_len;
   p.H = num_heads;
@@ -161,21 +199,26 @@ extern "C" int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_
   p.G = num_heads / kv_heads;
   p.Lkv = kv_len;
   p.Ls = shared_len;
+  p.by_lq = fast_div(q_len);
+  p.by_g = fast_div(p.G);
+  p.by_h = fast_div(num_heads);
+  p.by_hkv = fast_div(kv_heads);
   p.slots = plan.slots;
+  p.prows = plan.prows;
+  p.tail_rows = plan.tail_rows;
   p.o_part = static_cast<float*>(workspace);
-  p.ml_part = plan.slots > 1 ? reinterpret_cast<float2*>(p.o_part + (size_t)plan.slots * batch * q_len * num_heads *
-                                                                        head_dim)
-                             : nullptr;
+  if (plan.bytes) p.ml_part = reinterpret_cast<float2*>(p.o_part + (size_t)plan.slots * plan.prows * head_dim);
   const bool fp16 = dtype == HB_FP16;
   for (int kernel = 0; kernel < 2; ++kernel) {  // the parts of the few-rows kernel, then those of the tcgen05 one
     for (int i = 0; i < 2; ++i) {
       p.part[i] = plan.part[i];
-      if (plan.tiles[i] != (kernel == 1)) p.part[i].ctas = 0;
+      if (plan.tiles[i] != (kernel == 1)) p.part[i].count = 0;
     }
-    if (p.part[0].ctas + p.part[1].ctas == 0) continue;
+    if (p.part[0].count + p.part[1].count == 0) continue;
     const int rc = kernel ? launch_ctx_tiles(p, head_dim, fp16, plan.mask_tiles, stream)
                           : launch_ctx_rows(p, head_dim, fp16, plan.rows_per_tile, stream);
     if (rc != HB_OK) return rc;
   }
+  p.part[1] = plan.part[1];
   return plan.slots > 1 ? launch_ctx_combine(p, head_dim, fp16, stream) : HB_OK;
 }

@@ -87,19 +87,10 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
 
   // ---- which item
-  int idx = blockIdx.x;
-  const bool second = idx >= p.part[0].ctas;
-  const CtxPart& part = second ? p.part[1] : p.part[0];
-  if (second) idx -= p.part[0].ctas;
-  const int split = idx % part.splits;
-  idx /= part.splits;
-  const int rt = idx % part.row_tiles;
-  idx /= part.row_tiles;
-  const int g = idx % p.Hkv;
-  const int b = idx / p.Hkv;  // 0 for pooled items
-  const int rows = (part.pooled ? p.B : 1) * p.Lq * p.G;
-  const int tok0 = part.pooled ? 0 : b * p.Lq;
-  const int r0 = rt * 16 * MT;
+  const bool second = static_cast<int>(blockIdx.x) >= p.part[0].count;
+  const CtxPart& part = p.part[second ? 1 : 0];
+  const CtxUnit u = ctx_unit(p, part, blockIdx.x - (second ? p.part[0].count : 0));
+  const int g = u.g, b = u.b, r0 = u.rt * 16 * MT;
 
   // ---- query fragments (a row's RMSNorm when asked for, rounded to the input's type like the norm it replaces)
   uint32_t qf[MT][KK][4];
@@ -108,10 +99,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const int r = r0 + mt * 16 + hf * 8 + gid;
-      const bool live = r < rows;
-      const int tk = live ? r / p.G : 0, hq = g * p.G + (live ? r - tk * p.G : 0);
-      const int t = tok0 + tk, bq = t / p.Lq;
-      const uint16_t* src = p.q + bq * p.q_bs + (t - bq * p.Lq) * p.q_rs + (int64_t)hq * D;
+      const bool live = r < u.rows;
+      const CtxRow x = ctx_row(p, live ? r : 0, g, b, part.pooled);
+      const uint16_t* src = p.q + x.bq * p.q_bs + x.i * p.q_rs + (int64_t)x.hq * D;
       float ss = 0.f;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
@@ -142,8 +132,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
   const int own_len = part.use_own ? ctx_own_len(p, b) : 0;
   const int n0 = part.use_shared ? (p.Ls + KC - 1) / KC : 0;
   const int n = n0 + (own_len + KC - 1) / KC;
-  const int c_begin = static_cast<int>((int64_t)split * n / part.splits);
-  const int c_end = static_cast<int>((int64_t)(split + 1) * n / part.splits);
+  const int c_begin = part.by_splits.div(u.split * n);
+  const int c_end = part.by_splits.div((u.split + 1) * n);
   const uint32_t ring = smem_u32(smem) + warp * kWarpBytes;
   uint32_t* bits_w = bits_s + warp * kStages;
 
@@ -316,10 +306,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
         *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[mt][i][hf * 2], o[mt][i][hf * 2 + 1]);
     }
   __syncthreads();
-  const int64_t rall = (int64_t)p.B * p.Lq * p.H;
   for (int i = threadIdx.x; i < kRows * PPR; i += 32 * kWarps) {
     const int row = i / PPR, ch = i % PPR, r = r0 + row;
-    if (r >= rows) continue;
+    if (r >= u.rows) continue;
     float mw[kWarps], mx = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, mw[w] = ml_s[w * 32 + row].x);
@@ -332,18 +321,17 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc[e] = fmaf(f, src[e], acc[e]);
     }
-    const int tk = r / p.G, hq = g * p.G + (r - tk * p.G), t = tok0 + tk;
-    if (p.slots == 1) {
-      const int bq = t / p.Lq;
+    const CtxRow x = ctx_row(p, r, g, b, part.pooled);
+    if (part.direct) {
       const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
       uint4 w;
       w.x = T::pack(acc[0] * inv, acc[1] * inv);
       w.y = T::pack(acc[2] * inv, acc[3] * inv);
       w.z = T::pack(acc[4] * inv, acc[5] * inv);
       w.w = T::pack(acc[6] * inv, acc[7] * inv);
-      *reinterpret_cast<uint4*>(p.out + bq * p.o_bs + (t - bq * p.Lq) * p.o_rs + (int64_t)hq * D + ch * 8) = w;
+      *reinterpret_cast<uint4*>(p.out + x.bq * p.o_bs + x.i * p.o_rs + (int64_t)x.hq * D + ch * 8) = w;
     } else {
-      const int64_t pr = (part.slot0 + split) * rall + (int64_t)t * p.H + hq;
+      const int64_t pr = ctx_prow(p, part, u, x, row);
       if (ch == 0) p.ml_part[pr] = make_float2(mx, sum);
       float4* dst = reinterpret_cast<float4*>(p.o_part + pr * D + ch * 8);
       dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -356,20 +344,33 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
 template <int D, class T>
 __global__ void __launch_bounds__(256) ctx_combine_kernel(const CtxParams p) {
   constexpr int TPR = D / 4;
-  const int64_t rall = (int64_t)p.B * p.Lq * p.H;
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / TPR;
+  const int row = static_cast<int>(((int64_t)blockIdx.x * 256 + threadIdx.x) / TPR);
   const int ch = threadIdx.x % TPR;
-  if (row >= rall) return;
+  if (row >= p.prows) return;
+  CtxRow x;
+  if (p.tail_rows) {
+    const CtxPart& part = p.part[1];
+    const int i = row / p.tail_rows;
+    const CtxUnit u = ctx_unit(p, part, i * part.splits);
+    const int r = u.rt * p.tail_rows + (row - i * p.tail_rows);
+    if (r >= u.rows) return;
+    x = ctx_row(p, r, u.g, u.b, part.pooled);
+  } else {
+    const int t = p.by_h.div(row);
+    x.hq = row - t * p.H;
+    x.bq = p.by_lq.div(t);
+    x.i = t - x.bq * p.Lq;
+  }
   float mx = -INFINITY;
-  for (int s = 0; s < p.slots; ++s) mx = fmaxf(mx, p.ml_part[s * rall + row].x);
+  for (int s = 0; s < p.slots; ++s) mx = fmaxf(mx, p.ml_part[(int64_t)s * p.prows + row].x);
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int s = 0; s < p.slots; ++s) {
-    const float2 ml = p.ml_part[s * rall + row];
+    const float2 ml = p.ml_part[(int64_t)s * p.prows + row];
     if (ml.x == -INFINITY) continue;  // a part without keys left its sums unwritten
     const float f = ex2_approx(ml.x - mx);
-    const float4 v = *reinterpret_cast<const float4*>(p.o_part + (s * rall + row) * D + ch * 4);
+    const float4 v = *reinterpret_cast<const float4*>(p.o_part + ((int64_t)s * p.prows + row) * D + ch * 4);
     sum = fmaf(f, ml.y, sum);
     acc.x = fmaf(f, v.x, acc.x);
     acc.y = fmaf(f, v.y, acc.y);
@@ -377,13 +378,10 @@ __global__ void __launch_bounds__(256) ctx_combine_kernel(const CtxParams p) {
     acc.w = fmaf(f, v.w, acc.w);
   }
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-  const int64_t t = row / p.H;
-  const int hq = static_cast<int>(row - t * p.H);
-  const int64_t bq = t / p.Lq;
   uint2 w;
   w.x = T::pack(acc.x * inv, acc.y * inv);
   w.y = T::pack(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(p.out + bq * p.o_bs + (t - bq * p.Lq) * p.o_rs + (int64_t)hq * D + ch * 4) = w;
+  *reinterpret_cast<uint2*>(p.out + x.bq * p.o_bs + x.i * p.o_rs + (int64_t)x.hq * D + ch * 4) = w;
 }
 
 template <int D, class T, int MT>
@@ -391,13 +389,13 @@ int launch_rows(const CtxParams& p, cudaStream_t s) {
   if (cudaFuncSetAttribute(ctx_rows_kernel<D, T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem) !=
       cudaSuccess)
     return HB_ERR_LAUNCH;
-  ctx_rows_kernel<D, T, MT><<<p.part[0].ctas + p.part[1].ctas, 32 * kWarps, kRowsSmem, s>>>(p);
+  ctx_rows_kernel<D, T, MT><<<p.part[0].count + p.part[1].count, 32 * kWarps, kRowsSmem, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 
 template <int D, class T>
 int launch_combine(const CtxParams& p, cudaStream_t s) {
-  const int64_t threads = (int64_t)p.B * p.Lq * p.H * (D / 4);
+  const int64_t threads = (int64_t)p.prows * (D / 4);
   ctx_combine_kernel<D, T><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }

@@ -1,16 +1,20 @@
 // Context attention for many query rows: tcgen05 MMAs on 128-row x 128-key tiles.
 //
 // One CTA takes 128 rows of one kv head (a row: a query token and one query head of the group) and walks its keys:
-// S = Q K^T (fp32, TMEM), P = exp2(c S - m) (16-bit, back into TMEM over S), O += P V (fp32, TMEM), with the running
-// maximum m and sum of each row in the registers of one thread. The exponentials bound it (one per score against
-// 4 D flops: at D 64 the MUFU unit needs 1,024 cycles per tile and SM, the tensor pipe about 660), and within a
-// tile the three steps wait for one another. So two CTAs share an SM, each with 256 TMEM columns: one's softmax runs
-// while the other's MMAs do. A lazy maximum (O is rescaled only when a row's maximum grows by more than 2^8) keeps
-// O in TMEM, and a quarter of the exponentials goes to the FMA pipe (exp2_poly2).
+// S = Q K^T (fp32, TMEM), P = exp2(c S - m) (16-bit, TMEM), O += P V (fp32, TMEM), with the running maximum m and sum
+// of each row in the registers of one thread. The exponentials bound it (one per score against 4 D flops), and
+// one row per thread leaves each SM sub-partition a single softmax warp, which cannot fill its pipes. So two CTAs
+// share an SM, each with 256 TMEM columns. A lazy maximum (O is rescaled only when a row's maximum grows by more than
+// 2^8) keeps O in TMEM, and a quarter of the exponentials goes to the FMA pipe (exp2_poly2).
+// At D 64 P has columns of its own, so the next tile's S runs while this one's softmax does; at D 128 the columns are
+// taken (S 128, O 128), P lies over S and the other CTA fills the wait.
+//
+// The grid is one round of CTAs; each walks its share of the units (tiles of rows), so barriers, TMEM and tensor maps
+// are set up once, K and V of the next unit are on their way early and its queries during the epilogue.
 //
 // Roles (8 warps): warps 0-3 load and norm the queries, then the softmax (one row per thread) and the epilogue;
 // warp 4 TMA of K and V tiles (128-byte swizzle, rows past the end read as zero); warp 5 TMEM allocation and the one
-// MMA-issuing thread; warps 4-7 read the mask first. setmaxnreg moves registers from warps 4-7 to the softmax.
+// MMA-issuing thread; warp 6 reads the mask, one unit ahead. setmaxnreg moves registers from warps 4-7 to the softmax.
 // Keys that are not valid: their scores are set to -inf, and in a tile that has some inside the tensor their V rows
 // are zeroed in shared memory (0 * NaN would reach O); tiles without any valid key are skipped by every role.
 //
@@ -31,24 +35,26 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kLaunchRegs = 128;                 // 2 CTAs x 256 threads x 128 = the SM's 65,536
-constexpr int kSoftmaxRegs = 200, kOtherRegs = 56;
+constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
 static_assert(kSoftmaxRegs + kOtherRegs == 2 * kLaunchRegs, "the warpgroups share what the CTA was launched with");
 constexpr int kAtom = 128 * 128;                 // 128 rows of 128 bytes: 64 columns of a tile
 constexpr float kRescaleThreshold = 8.0f;        // log2 units
-constexpr int kTmemCols = 256;                   // S (P over it) at 0, O at 128
+constexpr int kTmemCols = 256;
 
 template <int D>
 struct Layout {
   static constexpr int kHalves = D / 64;
   static constexpr int kTile = kHalves * kAtom;
   static constexpr int kStages = D == 64 ? 2 : 1;
-  static constexpr int kOffK = kTile;                       // queries (the output is staged there too) at 0
+  static constexpr bool kOwnP = D == 64;                    // P beside S, not over it
+  static constexpr int kTmemP = kOwnP ? 128 : 0, kTmemO = kOwnP ? 192 : 128;  // columns; S at 0
+  static constexpr int kOffK = kTile;                       // queries at 0
   static constexpr int kOffV = kOffK + kStages * kTile;
   static constexpr int kOffBars = kOffV + kStages * kTile;
-  static constexpr int kBars = 4 * kStages + 4;
+  static constexpr int kBars = 4 * kStages + 10;
   static constexpr int kOffMisc = kOffBars + kBars * 8;     // TMEM address, abort flag
   static constexpr int kOffBits = (kOffMisc + 8 + 15) & ~15;
-  static constexpr int bytes(int mask_tiles) { return kOffBits + mask_tiles * 16 + 1024; }
+  static constexpr int bytes(int mask_tiles) { return kOffBits + 2 * mask_tiles * 16 + 1024; }
 };
 static_assert(Layout<64>::bytes(kCtxMaskTiles) <= 113 * 1024 && Layout<128>::bytes(kCtxMaskTiles) <= 113 * 1024,
               "two CTAs per SM");
@@ -76,44 +82,76 @@ constexpr uint32_t idesc_base(bool b_mn_major) {
 }
 __device__ __forceinline__ uint32_t idesc_n(uint32_t base, int n) { return base | (static_cast<uint32_t>(n >> 3) << 17); }
 
-__device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (mbar_wait(bar, parity) && !*abort_flag) return true;
+// Bounded waits (one second) that end early once another role has given up.
+__device__ __forceinline__ bool slow_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!*abort_flag) {
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      record_error(HB_ERR_TIMEOUT);
+      break;
+    }
+  }
   *abort_flag = 1;
   return false;
 }
+__device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return mbar_try_wait(bar, parity) || slow_wait(bar, parity, abort_flag);
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity) && !*abort_flag);
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || slow_wait(bar, parity, abort_flag));
 }
 
-// A tile of the key list: keys [k0, k0 + 128) of the shared states or of the batch element's own. `hi` counts the
-// keys up to the last one that may be valid (0: skip the tile); with a mask, bits says which are.
+// A unit's key list: tiles [j0, j1) of the shared states' n0 tiles, then the batch element's own.
+struct Keys {
+  int n0, own_len, j0, j1;
+};
+__device__ __forceinline__ Keys keys_of(const CtxParams& p, const CtxPart& part, const CtxUnit& u) {
+  Keys k;
+  k.own_len = part.use_own ? ctx_own_len(p, u.b) : 0;
+  k.n0 = part.use_shared ? (p.Ls + 127) >> 7 : 0;
+  const int n = k.n0 + ((k.own_len + 127) >> 7);
+  k.j0 = part.by_splits.div(u.split * n);
+  k.j1 = part.by_splits.div((u.split + 1) * n);
+  return k;
+}
+
+// Keys [k0, k0 + 128) of either. `hi` counts them up to the last one that may be valid (0: skip the tile); with a
+// mask, bits says which are.
 struct Tile {
   int k0, hi;
   bool shared, full, clean;  // full: all 128 valid; clean: some of the tensor's rows in [0, hi) must not be read
   uint4 bits;
 };
-
 template <bool kMask>
-__device__ __forceinline__ Tile tile_of(const CtxParams& p, int j, int n0, int own_len, const uint4* bits, int j0) {
+__device__ __forceinline__ Tile tile_of(const CtxParams& p, const Keys& ks, int j, const uint4* bits) {
   Tile t;
-  t.shared = j < n0;
-  t.k0 = (t.shared ? j : j - n0) * 128;
-  t.hi = min(128, (t.shared ? p.Ls : own_len) - t.k0);
-  t.full = t.hi == 128;
-  // rows between hi and the next multiple of 16 enter P V: zeros past the tensor, anything before its end
-  t.clean = !t.shared && (t.hi & 15) && own_len < p.Lkv;
+  t.shared = j < ks.n0;
+  t.k0 = (t.shared ? j : j - ks.n0) * 128;
   if constexpr (kMask) {
-    t.bits = bits[j - j0];
+    t.bits = bits[j - ks.j0];
     const uint32_t b[4] = {t.bits.x, t.bits.y, t.bits.z, t.bits.w};
-    int hi = 0;
+    t.hi = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (b[i]) hi = 32 * i + 32 - __clz(b[i]);
-    t.hi = hi;
+      if (b[i]) t.hi = 32 * i + 32 - __clz(b[i]);
     t.full = (b[0] & b[1] & b[2] & b[3]) == 0xffffffffu;
     t.clean = !t.full;
+  } else {
+    t.hi = min(128, (t.shared ? p.Ls : ks.own_len) - t.k0);
+    t.full = t.hi == 128;
+    // rows between hi and the next multiple of 16 enter P V: zeros past the tensor, anything before its end
+    t.clean = !t.shared && (t.hi & 15) && ks.own_len < p.Lkv;
   }
   return t;
+}
+
+// One aligned 32-byte sector.
+__device__ __forceinline__ void st_32b(void* dst, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4& b, int i) {
@@ -123,7 +161,7 @@ __device__ __forceinline__ uint32_t word_of(const uint4& b, int i) {
 template <int D, bool kFp16, bool kMask>
 __global__ void __launch_bounds__(kThreads, 2)
     ctx_tiles_kernel(const __grid_constant__ CUtensorMap tm_own, const __grid_constant__ CUtensorMap tm_shared,
-                     const CtxParams p) {
+                     const __grid_constant__ CtxParams p, const int mask_tiles) {
   using L = Layout<D>;
   constexpr int kStages = L::kStages;
   constexpr int PPR = D / 8;  // 16-byte pieces per row
@@ -135,35 +173,23 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* k_empty = k_full + kStages;     // [kStages] commit of the S MMAs
   uint64_t* v_full = k_empty + kStages;     // [kStages] TMA bytes
   uint64_t* v_empty = v_full + kStages;     // [kStages] commit of the P V MMAs
-  uint64_t* q_full = v_empty + kStages;     // 4 softmax warps wrote the queries
-  uint64_t* s_full = q_full + 1;            // commit: S written (and the tile before's P V done)
-  uint64_t* p_ready = s_full + 1;           // 4 softmax warps wrote P
-  uint64_t* o_full = p_ready + 1;           // commit: everything done
+  uint64_t* q_full = v_empty + kStages;     // 4 softmax warps wrote the queries (units that have keys)
+  uint64_t* s_full = q_full + 1;            // commit: S written
+  uint64_t* s_free = s_full + 1;            // 4 softmax warps loaded S (kOwnP)
+  uint64_t* p_ready = s_free + 1;           // 4 softmax warps wrote P
+  uint64_t* o_done = p_ready + 1;           // commit: the tile's P V added
+  uint64_t* drain = o_done + 1;
+  uint64_t* m_full = drain + 1;             // [2] warp 6 wrote the unit's mask bits
+  uint64_t* m_free = m_full + 2;            // [2] the six roles' warps are through with them
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
-  uint4* bits = reinterpret_cast<uint4*>(smem + L::kOffBits);
+  uint4* bits0 = reinterpret_cast<uint4*>(smem + L::kOffBits);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int count0 = p.part[0].count, total = count0 + p.part[1].count;
 
-  // ---- which item
-  int idx = blockIdx.x;
-  const bool second = idx >= p.part[0].ctas;
-  const CtxPart& part = second ? p.part[1] : p.part[0];
-  if (second) idx -= p.part[0].ctas;
-  const int split = idx % part.splits;
-  idx /= part.splits;
-  const int rt = idx % part.row_tiles;
-  idx /= part.row_tiles;
-  const int g = idx % p.Hkv;
-  const int b = idx / p.Hkv;  // 0 for pooled items
-  const int rows = (part.pooled ? p.B : 1) * p.Lq * p.G;
-  const int tok0 = part.pooled ? 0 : b * p.Lq;
-  const int own_len = part.use_own ? ctx_own_len(p, b) : 0;
-  const int n0 = part.use_shared ? (p.Ls + 127) / 128 : 0;
-  const int n = n0 + (own_len + 127) / 128;
-  const int j0 = static_cast<int>((int64_t)split * n / part.splits);
-  const int j1 = static_cast<int>((int64_t)(split + 1) * n / part.splits);
-
-  if (threadIdx.x == 0) {
+  if (warp == 4 && lane == 0) {
+    prefetch_tmap(&tm_own);
+    prefetch_tmap(&tm_shared);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -172,8 +198,14 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     mbar_init(q_full, 4);
     mbar_init(s_full, 1);
+    mbar_init(s_free, 4);
     mbar_init(p_ready, 4);
-    mbar_init(o_full, 1);
+    mbar_init(o_done, 1);
+    mbar_init(drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&m_full[i], 1);
+      mbar_init(&m_free[i], 6);
+    }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -181,38 +213,31 @@ __global__ void __launch_bounds__(kThreads, 2)
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
-  if (kMask && warp >= 4) {
-    for (int j = j0 + warp - 4; j < j1; j += 4) {
-      const bool sh = j < n0;
-      const int k0 = (sh ? j : j - n0) * 128, len = sh ? p.Ls : own_len;
-      const uint8_t* mk = sh ? p.smask : (p.mask ? p.mask + b * p.mask_bs : nullptr);
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = k0 + 32 * i + lane;
-        bool v = k < len;
-        if (v && mk) v = mk[k] != 0;
-        w[i] = __ballot_sync(0xffffffffu, v);
-      }
-      if (lane == 0) bits[j - j0] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-  // The queries are on their way while the CTA sets up: a row's PPR pieces in PPR consecutive lanes.
+  // Work unit w's queries, asynchronously into the shared-memory image (rows past the end as zeros): warp i its 32
+  // rows, a row's PPR pieces by PPR consecutive lanes.
   constexpr int kRowsPerStep = 32 / PPR, kSteps = 32 / kRowsPerStep;
-  uint4 qv[kSteps];
-  const int qch = lane % PPR;
-  if (warp < 4) {
+  const int qch = lane % PPR, qrow = warp * 32 + lane / PPR;
+  auto load_q = [&](int w) {
+    const CtxPart& part = p.part[w >= count0 ? 1 : 0];
+    const CtxUnit u = ctx_unit(p, part, w - (w >= count0 ? count0 : 0));
+    const bool plain = p.G == 1 && !part.pooled;  // rows one stride apart
+    const uint16_t* src = p.q + (plain ? u.b * p.q_bs + (int64_t)(u.rt * 128 + qrow) * p.q_rs + u.g * D : 0) + qch * 8;
+    const uint32_t dst = smem_u32(smem) + (qch >> 3) * kAtom;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      const int r = rt * 128 + warp * 32 + i * kRowsPerStep + lane / PPR;
-      qv[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows) {
-        const int tk = r / p.G, hq = g * p.G + (r - tk * p.G), t = tok0 + tk, bq = t / p.Lq;
-        qv[i] = __ldg(reinterpret_cast<const uint4*>(p.q + bq * p.q_bs + (t - bq * p.Lq) * p.q_rs + (int64_t)hq * D +
-                                                     qch * 8));
+      const int lr = qrow + i * kRowsPerStep, r = u.rt * 128 + lr;
+      const bool live = r < u.rows;
+      const uint16_t* from = src + i * kRowsPerStep * p.q_rs;
+      if (!plain) {
+        const CtxRow x = ctx_row(p, live ? r : 0, u.g, u.b, part.pooled);
+        from = src + x.bq * p.q_bs + x.i * p.q_rs + x.hq * D;
       }
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + sw128_offset(lr, qch & 7)),
+                   "l"(live ? from : p.q), "r"(live ? 16u : 0u) : "memory");
     }
-  }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (warp < 4) load_q(blockIdx.x);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -223,30 +248,39 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (warp == 4 && lane == 0) {
       // -------------------------------------------------------------- TMA producer
       int it = 0;
-      const int kcol = g * D, vcol = p.Hkv * D + g * D;
-      for (int j = j0; j < j1; ++j) {
-        const Tile t = tile_of<kMask>(p, j, n0, own_len, bits, j0);
-        if (t.hi <= 0) continue;
-        const int st = it % kStages;
-        const uint32_t ph = ((it / kStages) & 1) ^ 1;
-        const CUtensorMap* tm = t.shared ? &tm_shared : &tm_own;
-        const bool inter = !t.shared && p.kv_inter;  // the map's second dimension is the batch
-        const int bc = t.shared || p.kv_bs == 0 ? 0 : b;
-        const int c1 = inter ? bc : t.k0, c2 = inter ? t.k0 : bc;
-        if (it >= kStages && !role_wait(&k_empty[st], ph, abort_flag)) break;
-        mbar_arrive_expect_tx(&k_full[st], L::kTile);
+      bool ok = true;
+      for (int n = 0, w = blockIdx.x; ok && w < total; ++n, w += gridDim.x) {
+        const CtxPart& part = p.part[w >= count0 ? 1 : 0];
+        const CtxUnit u = ctx_unit(p, part, w - (w >= count0 ? count0 : 0));
+        const Keys ks = keys_of(p, part, u);
+        const uint4* bits = bits0 + (n & 1) * mask_tiles;
+        const int kcol = u.g * D, vcol = p.Hkv * D + u.g * D;
+        if (kMask && !(ok = role_wait(&m_full[n & 1], (n >> 1) & 1, abort_flag))) break;
+        for (int j = ks.j0; j < ks.j1; ++j) {
+          const Tile t = tile_of<kMask>(p, ks, j, bits);
+          if (t.hi <= 0) continue;
+          const int st = it % kStages;
+          const uint32_t ph = ((it / kStages) & 1) ^ 1;
+          const CUtensorMap* tm = t.shared ? &tm_shared : &tm_own;
+          const bool inter = !t.shared && p.kv_inter;  // the map's second dimension is the batch
+          const int bc = t.shared || p.kv_bs == 0 ? 0 : u.b;
+          const int c1 = inter ? bc : t.k0, c2 = inter ? t.k0 : bc;
+          if (it >= kStages && !(ok = role_wait(&k_empty[st], ph, abort_flag))) break;
+          mbar_arrive_expect_tx(&k_full[st], L::kTile);
 #pragma unroll
-        for (int h = 0; h < L::kHalves; ++h)
-          tma_load_3d(smem + L::kOffK + st * L::kTile + h * kAtom, tm, kcol + 64 * h, c1, c2, &k_full[st]);
-        if (it >= kStages && !role_wait(&v_empty[st], ph, abort_flag)) {
-          mbar_wait(&k_full[st], (it / kStages) & 1);
-          break;
+          for (int h = 0; h < L::kHalves; ++h)
+            tma_load_3d(smem + L::kOffK + st * L::kTile + h * kAtom, tm, kcol + 64 * h, c1, c2, &k_full[st]);
+          if (it >= kStages && !(ok = role_wait(&v_empty[st], ph, abort_flag))) {
+            mbar_wait(&k_full[st], (it / kStages) & 1);  // K was issued already
+            break;
+          }
+          mbar_arrive_expect_tx(&v_full[st], L::kTile);
+#pragma unroll
+          for (int h = 0; h < L::kHalves; ++h)
+            tma_load_3d(smem + L::kOffV + st * L::kTile + h * kAtom, tm, vcol + 64 * h, c1, c2, &v_full[st]);
+          ++it;
         }
-        mbar_arrive_expect_tx(&v_full[st], L::kTile);
-#pragma unroll
-        for (int h = 0; h < L::kHalves; ++h)
-          tma_load_3d(smem + L::kOffV + st * L::kTile + h * kAtom, tm, vcol + 64 * h, c1, c2, &v_full[st]);
-        ++it;
+        if (kMask) mbar_arrive(&m_free[n & 1]);
       }
       // every copy issued into this CTA's shared memory lands before it exits
       for (int i = max(0, it - kStages); i < it; ++i) {
@@ -255,227 +289,291 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     } else if (warp == 5 && lane == 0) {
       // -------------------------------------------------------------- MMA issuer
-      constexpr uint32_t idS = idesc_base<kFp16>(false), idO = idesc_base<kFp16>(true);
-      const uint32_t qa = smem_u32(smem), kb0 = smem_u32(smem + L::kOffK), vb0 = smem_u32(smem + L::kOffV);
-      const uint32_t tS = tmem, tO = tmem + 128;
-      int it = 0;
-      for (int j = j0; j < j1; ++j) {
-        const Tile t = tile_of<kMask>(p, j, n0, own_len, bits, j0);
-        if (t.hi <= 0) continue;
-        const int st = it % kStages, n16 = (t.hi + 15) & ~15;
-        if (it == 0 && !role_wait(q_full, 0, abort_flag)) break;
-        if (!role_wait(&k_full[st], (it / kStages) & 1, abort_flag)) break;
+      constexpr uint32_t idS = idesc_base<kFp16>(false), idO = idesc_base<kFp16>(true) | ((D >> 3) << 17);
+      const uint64_t dq = smem_desc_sw128(smem_u32(smem));
+      const uint64_t dk = smem_desc_sw128(smem_u32(smem + L::kOffK));
+      // V tiles are MN-major: 16 keys are 2,048 bytes on, the second 64 columns one atom on
+      const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kOffV), D == 64 ? 16 : kAtom);
+      const uint32_t tS = tmem, tP = tmem + L::kTmemP, tO = tmem + L::kTmemO;
+      int it = 0, units = 0;
+      auto issue_s = [&](int i, int n16) {
+        const int st = i % kStages;
+        if (L::kOwnP && i > 0 && !role_wait(s_free, (i - 1) & 1, abort_flag)) return false;
+        if (!role_wait(&k_full[st], (i / kStages) & 1, abort_flag)) return false;
         tc_fence_after();
-        const uint32_t kb = kb0 + st * L::kTile, vb = vb0 + st * L::kTile;
-        const uint32_t id = idesc_n(idS, n16);
+        const uint32_t id = idS | (static_cast<uint32_t>(n16 >> 3) << 17);
+        const uint64_t kd = dk + st * (L::kTile >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k / 4) * kAtom + (k % 4) * 32;
-          mma_bf16_ss(tS, smem_desc_sw128(qa + off), smem_desc_sw128(kb + off), id, k > 0);
+          const uint32_t off = ((k / 4) * kAtom + (k % 4) * 32) >> 4;
+          mma_bf16_ss(tS, dq + off, kd + off, id, k > 0);
         }
         tc_commit(s_full);
         tc_commit(&k_empty[st]);
-        if (!role_wait(p_ready, it & 1, abort_flag)) break;
-        if (!role_wait(&v_full[st], (it / kStages) & 1, abort_flag)) break;
-        tc_fence_after();
-        // V tiles are MN-major: 16 keys are 2,048 bytes on, the second 64 columns one atom on
-        for (int k = 0; k < n16 / 16; ++k)
-          mma_bf16_ts(tO, tS + 8 * k, smem_desc_sw128(vb + 2048 * k, D == 64 ? 16 : kAtom), idesc_n(idO, D),
-                      it > 0 || k > 0);
-        tc_commit(&v_empty[st]);
-        ++it;
+        return true;
+      };
+      bool ok = true;
+      for (int n = 0, w = blockIdx.x; ok && w < total; ++n, w += gridDim.x) {
+        const CtxPart& part = p.part[w >= count0 ? 1 : 0];
+        const Keys ks = keys_of(p, part, ctx_unit(p, part, w - (w >= count0 ? count0 : 0)));
+        const uint4* bits = bits0 + (n & 1) * mask_tiles;
+        if (kMask && !(ok = role_wait(&m_full[n & 1], (n >> 1) & 1, abort_flag))) break;
+        auto next_tile = [&](int j, int& n16) {  // the first tile at or after j that has valid keys
+          for (; j < ks.j1; ++j) {
+            const Tile t = tile_of<kMask>(p, ks, j, bits);
+            n16 = (t.hi + 15) & ~15;
+            if (t.hi > 0) break;
+          }
+          return j;
+        };
+        int n16 = 0, n16_next = 0;
+        int j = next_tile(ks.j0, n16);
+        if (j < ks.j1) ok = role_wait(q_full, units++ & 1, abort_flag) && issue_s(it, n16);
+        for (bool first = true; ok && j < ks.j1; first = false) {
+          const int jn = next_tile(j + 1, n16_next), st = it % kStages;
+          // P beside S: the next S while the softmax computes this tile's P
+          if (L::kOwnP && jn < ks.j1 && !(ok = issue_s(it + 1, n16_next))) break;
+          if (!(ok = role_wait(&v_full[st], (it / kStages) & 1, abort_flag) && role_wait(p_ready, it & 1, abort_flag)))
+            break;
+          tc_fence_after();
+          const uint64_t vd = dv + st * (L::kTile >> 4);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (16 * k < n16) mma_bf16_ts(tO, tP + 8 * k, vd + k * (2048 >> 4), idO, !first || k > 0);
+          tc_commit(o_done);
+          tc_commit(&v_empty[st]);
+          // P over S: in the tensor pipe's order, P V reads P before the next S overwrites it
+          if (!L::kOwnP && jn < ks.j1 && !(ok = issue_s(it + 1, n16_next))) break;
+          ++it;
+          j = jn;
+          n16 = n16_next;
+        }
+        if (kMask) mbar_arrive(&m_free[n & 1]);
       }
-      tc_commit(o_full);
-      mbar_wait(o_full, 0);  // every MMA this thread issued has finished before TMEM is freed
+      tc_commit(drain);  // every MMA this thread issued has finished before TMEM is freed
+      mbar_wait(drain, 0);
+    } else if (kMask && warp == 6) {
+      // -------------------------------------------------------------- mask bits, one unit ahead of their readers
+      for (int n = 0, w = blockIdx.x; w < total; ++n, w += gridDim.x) {
+        const CtxPart& part = p.part[w >= count0 ? 1 : 0];
+        const CtxUnit u = ctx_unit(p, part, w - (w >= count0 ? count0 : 0));
+        const Keys ks = keys_of(p, part, u);
+        uint4* bits = bits0 + (n & 1) * mask_tiles;
+        if (n >= 2 && !warp_wait(&m_free[n & 1], ((n >> 1) & 1) ^ 1, abort_flag)) break;
+        for (int j = ks.j0; j < ks.j1; ++j) {
+          const bool sh = j < ks.n0;
+          const int k0 = (sh ? j : j - ks.n0) * 128, len = sh ? p.Ls : ks.own_len;
+          const uint8_t* mk = sh ? p.smask : (p.mask ? p.mask + u.b * p.mask_bs : nullptr);
+          uint32_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = k0 + 32 * i + lane;
+            v[i] = k < len ? (mk ? mk[k] : 1u) : 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = __ballot_sync(0xffffffffu, v[i] != 0u);
+          if (lane == 0) bits[j - ks.j0] = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        if (lane == 0) mbar_arrive(&m_full[n & 1]);  // lane 0 wrote them all
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    // ---------------------------------------------------------------- queries into shared memory
-    if (p.q_w) {  // rounded to the input's type, as the norm pass that this replaces stores it
-      float w[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = __ldg(p.q_w + qch * 8 + e);
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        uint32_t u[4] = {qv[i].x, qv[i].y, qv[i].z, qv[i].w};
-        float2 f[4];
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          f[e] = unpack16<kFp16>(u[e]);
-          ss = fmaf(f[e].x, f[e].x, fmaf(f[e].y, f[e].y, ss));
-        }
-#pragma unroll
-        for (int o = 1; o < PPR; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = rsqrtf(ss * (1.f / D) + p.eps);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = pack16<kFp16>(f[e].x * inv * w[2 * e], f[e].y * inv * w[2 * e + 1]);
-        qv[i] = make_uint4(u[0], u[1], u[2], u[3]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int r = warp * 32 + i * kRowsPerStep + lane / PPR;
-      *reinterpret_cast<uint4*>(smem + (qch >> 3) * kAtom + sw128_offset(r, qch & 7)) = qv[i];
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(q_full);
-
-    // ---------------------------------------------------------------- softmax
     const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t tS = tmem + lane_base, tO = tmem + lane_base + 128;
+    const uint32_t tS = tmem + lane_base, tP = tS + L::kTmemP, tO = tS + L::kTmemO;
     const int row = warp * 32 + lane;
-    float m = -INFINITY, l = 0.f;
     int it = 0;
     bool ok = true;
-    for (int j = j0; j < j1; ++j) {
-      const Tile t = tile_of<kMask>(p, j, n0, own_len, bits, j0);
-      if (t.hi <= 0) continue;
-      if (!(ok = warp_wait(s_full, it & 1, abort_flag))) break;
-      tc_fence_after();
-      uint32_t r[4][32];
+    for (int n = 0, w = blockIdx.x; ok && w < total; ++n, w += gridDim.x) {
+      const CtxPart& part = p.part[w >= count0 ? 1 : 0];
+      const CtxUnit u = ctx_unit(p, part, w - (w >= count0 ? count0 : 0));
+      const Keys ks = keys_of(p, part, u);
+      const uint4* bits = bits0 + (n & 1) * mask_tiles;
+      if (kMask && !(ok = warp_wait(&m_full[n & 1], (n >> 1) & 1, abort_flag))) break;
+      // -------------------------------------------------------------- queries: each lane's own pieces have landed
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (p.q_w) {  // rounded to the input's type, as the norm pass that this replaces stores it
+        float wv[8];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, r[c]);
-      tmem_wait_ld();
-      if (!t.full) {  // columns past n16 hold an earlier tile's bits
+        for (int e = 0; e < 8; ++e) wv[e] = __ldg(p.q_w + qch * 8 + e);
+#pragma unroll 2
+        for (int i = 0; i < kSteps; ++i) {
+          uint4* at = reinterpret_cast<uint4*>(smem + (qch >> 3) * kAtom + sw128_offset(qrow + i * kRowsPerStep, qch & 7));
+          const uint4 v = *at;
+          uint32_t x[4] = {v.x, v.y, v.z, v.w};
+          float2 f[4];
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[e] = unpack16<kFp16>(x[e]);
+            ss = fmaf(f[e].x, f[e].x, fmaf(f[e].y, f[e].y, ss));
+          }
+#pragma unroll
+          for (int o = 1; o < PPR; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float inv = rsqrtf(ss * (1.f / D) + p.eps);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = pack16<kFp16>(f[e].x * inv * wv[2 * e], f[e].y * inv * wv[2 * e + 1]);
+          *at = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+
+      // -------------------------------------------------------------- softmax
+      float m = -INFINITY, l = 0.f;
+      bool first = true;
+      for (int j = ks.j0; j < ks.j1; ++j) {
+        const Tile t = tile_of<kMask>(p, ks, j, bits);
+        if (t.hi <= 0) continue;
+        if (first && lane == 0) mbar_arrive(q_full);
+        if (!(ok = warp_wait(s_full, it & 1, abort_flag))) break;
+        tc_fence_after();
+        uint32_t r[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, r[c]);
+        tmem_wait_ld();
+        if constexpr (L::kOwnP) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free);
+        }
+        if (!t.full) {  // columns past hi hold an earlier tile's bits
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t word;
+            if constexpr (kMask) {
+              word = word_of(t.bits, c);
+            } else {
+              const int left = t.hi - 32 * c;
+              word = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((word >> e) & 1u)) r[c][e] = 0xff800000u;  // -inf
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            mx[c] = fmax3(mx[c], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+        const float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        const float m_new = fmaxf(m, rmax);
+        const bool upd = m_new > m + kRescaleThreshold;
+        float alpha = 1.f;
+        if (upd) {
+          alpha = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
+          m = m_new;
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+        float rs[4] = {0.f, 0.f, 0.f, 0.f};
+        // the tile before's P V has read P and written O
+        if (!first && !(ok = warp_wait(o_done, (it - 1) & 1, abort_flag))) break;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t word;
-          if constexpr (kMask) {
-            word = word_of(t.bits, c);
-          } else {
-            const int left = t.hi - 32 * c;
-            word = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1, p0, p1;
+            ffma2(x0, x1, __uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1]), p.scale_log2, p.scale_log2,
+                  nm, nm);
+            if ((e & kPolyMask) == kPolyMask) {  // a share of the exponentials on the FMA pipe
+              exp2_poly2(x0, x1, p0, p1);
+            } else {
+              p0 = ex2_approx(x0);
+              p1 = ex2_approx(x1);
+            }
+            const int a2 = (e & 1) * 2;
+            fadd2(rs[a2], rs[a2 + 1], rs[a2], rs[a2 + 1], p0, p1);
+            // P in the input's type for the MMA (at most 2^8 above 1, relative error up to 2^-8 or 2^-11)
+            pk[e] = pack16<kFp16>(p0, p1);
           }
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((word >> e) & 1u)) r[c][e] = 0xff800000u;  // -inf
+          tmem_st16(tP + 16 * c, pk);
         }
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        l = l * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
+        if (!first && __any_sync(0xffffffffu, upd)) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + 32 * c, o);
+            tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; e += 2)
-          mx[c] = fmax3(mx[c], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
-      const float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-      const float m_new = fmaxf(m, rmax);
-      const bool upd = m_new > m + kRescaleThreshold;
-      float alpha = 1.f;
-      if (upd) {
-        alpha = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
-        m = m_new;
-      }
-      const float nm = m == -INFINITY ? 0.f : -m;
-      float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float x0, x1, p0, p1;
-          ffma2(x0, x1, __uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1]), p.scale_log2, p.scale_log2,
-                nm, nm);
-          if ((e & kPolyMask) == kPolyMask) {  // a share of the exponentials on the FMA pipe
-            exp2_poly2(x0, x1, p0, p1);
-          } else {
-            p0 = ex2_approx(x0);
-            p1 = ex2_approx(x1);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(tO + 32 * c, o);
           }
-          const int a2 = (e & 1) * 2;
-          fadd2(rs[a2], rs[a2 + 1], rs[a2], rs[a2 + 1], p0, p1);
-          // P in the input's type for the MMA (at most 2^8 above 1, relative error up to 2^-8 or 2^-11)
-          pk[e] = pack16<kFp16>(p0, p1);
         }
-        tmem_st16(tS + 16 * c, pk);
+        if (t.clean) {  // this thread's V row, where its key is not valid
+          const int st = it % kStages;
+          if (!(ok = warp_wait(&v_full[st], (it / kStages) & 1, abort_flag))) break;
+          bool valid = row < t.hi;
+          if constexpr (kMask) valid = (word_of(t.bits, warp) >> lane) & 1u;
+          if (!valid) {
+            uint8_t* v = smem + L::kOffV + st * L::kTile;
+#pragma unroll
+            for (int c = 0; c < PPR; ++c)
+              *reinterpret_cast<uint4*>(v + (c >> 3) * kAtom + sw128_offset(row, c & 7)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+        ++it;
+        first = false;
       }
-      l = l * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
-      if (it > 0 && __any_sync(0xffffffffu, upd)) {
+      if (kMask && lane == 0) mbar_arrive(&m_free[n & 1]);
+      // -------------------------------------------------------------- epilogue: one row per thread
+      if (!ok) break;
+      if (w + gridDim.x < total) load_q(w + gridDim.x);  // (the S MMAs of this unit are done)
+      if (!first && !(ok = warp_wait(o_done, (it - 1) & 1, abort_flag))) break;
+      tc_fence_after();
+      const int gr = u.rt * 128 + row;
+      const bool live = gr < u.rows;
+      const CtxRow x = ctx_row(p, live ? gr : 0, u.g, u.b, part.pooled);
+      if (part.direct) {
+        const float inv = l > 0.f ? 1.f / l : l;  // l 0: no key; NaN stays
+        uint16_t* dst = p.out + x.bq * p.o_bs + x.i * p.o_rs + x.hq * D;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32], v[16];
+          tmem_ld32(tO + 32 * c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            v[e] = l == 0.f ? 0u
+                            : pack16<kFp16>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+          if (live) {
+            if (p.out_wide) {  // whole 32-byte sectors
+              st_32b(dst + c * 32, v);
+              st_32b(dst + c * 32 + 16, v + 8);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) =
+                    make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            }
+          }
+        }
+      } else {
+        const int64_t pr = ctx_prow(p, part, u, x, row);
+        if (live) p.ml_part[pr] = make_float2(l == 0.f ? -INFINITY : m, l);
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(tO + 32 * c, o);
           tmem_wait_ld();
+          if (live) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st32(tO + 32 * c, o);
+            for (int e = 0; e < 4; ++e) st_32b(p.o_part + pr * D + c * 32 + e * 8, o + 8 * e);
+          }
         }
       }
-      if (t.clean) {  // this thread's V row, where its key is not valid
-        const int st = it % kStages;
-        if (!(ok = warp_wait(&v_full[st], (it / kStages) & 1, abort_flag))) break;
-        bool valid = row < t.hi;
-        if constexpr (kMask) valid = (word_of(t.bits, warp) >> lane) & 1u;
-        if (!valid) {
-          uint8_t* v = smem + L::kOffV + st * L::kTile;
-#pragma unroll
-          for (int c = 0; c < PPR; ++c)
-            *reinterpret_cast<uint4*>(v + (c >> 3) * kAtom + sw128_offset(row, c & 7)) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        fence_proxy_async_smem();
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_ready);
-      ++it;
+      tc_fence_before();  // O has been read; the next unit's first P V follows this warp's p_ready
     }
     if (!ok) *abort_flag = 1;
-
-    // ---------------------------------------------------------------- epilogue
-    ok = warp_wait(o_full, 0, abort_flag) && ok;
-    tc_fence_after();
-    const int r = rt * 128 + row;
-    if (p.slots == 1) {
-      const float inv = l > 0.f ? 1.f / l : l;  // l 0: no key; NaN stays
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(tO + 32 * c, o);
-        tmem_wait_ld();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float a = __uint_as_float(o[q * 8 + 2 * e]) * inv, z = __uint_as_float(o[q * 8 + 2 * e + 1]) * inv;
-            w[e] = l == 0.f ? 0u : pack16<kFp16>(a, z);
-          }
-          const int ch = c * 4 + q;
-          *reinterpret_cast<uint4*>(smem + (ch >> 3) * kAtom + sw128_offset(row, ch & 7)) =
-              make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {  // whole rows, coalesced
-        const int lr = warp * 32 + i * kRowsPerStep + lane / PPR, gr = rt * 128 + lr;
-        if (ok && gr < rows) {
-          const int tk = gr / p.G, hq = g * p.G + (gr - tk * p.G), tt = tok0 + tk, bq = tt / p.Lq;
-          *reinterpret_cast<uint4*>(p.out + bq * p.o_bs + (tt - bq * p.Lq) * p.o_rs + (int64_t)hq * D + qch * 8) =
-              *reinterpret_cast<const uint4*>(smem + (qch >> 3) * kAtom + sw128_offset(lr, qch & 7));
-        }
-      }
-    } else {
-      const int64_t rall = (int64_t)p.B * p.Lq * p.H;
-      const int tk = r / p.G;
-      const int64_t pr = (part.slot0 + split) * rall + (int64_t)(tok0 + tk) * p.H + g * p.G + (r - tk * p.G);
-      if (r < rows) p.ml_part[pr] = make_float2(l == 0.f ? -INFINITY : m, l);
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(tO + 32 * c, o);
-        tmem_wait_ld();
-        if (r < rows) {
-          float4* dst = reinterpret_cast<float4*>(p.o_part + pr * D + c * 32);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                 __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-        }
-      }
-    }
   }
   tc_fence_before();
   __syncthreads();
@@ -524,7 +622,8 @@ int launch_tiles(const CUtensorMap& own, const CUtensorMap& shared, const CtxPar
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::bytes(kCtxMaskTiles)) !=
       cudaSuccess)
     return HB_ERR_LAUNCH;
-  kernel<<<p.part[0].ctas + p.part[1].ctas, kThreads, Layout<D>::bytes(mask_tiles), s>>>(own, shared, p);
+  const int grid = std::min(p.part[0].count + p.part[1].count, kCtxRound);
+  kernel<<<grid, kThreads, Layout<D>::bytes(mask_tiles), s>>>(own, shared, p, mask_tiles);
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 

@@ -128,7 +128,7 @@ int hb_context_workspace_bytes(int batch, int q_len, int kv_len, int shared_len,
  * A row without a valid key is written as zeros; what lies at keys that are not valid (infinities, NaN) does not
  * reach the result. Scores, softmax statistics and sums are fp32; the weights p are rounded to the 16-bit type for
  * the product with v (relative error at most 2^-8 or 2^-11 each), the sum of p is not. head_dim 64 or 128; rows of q, kv,
- * shared_kv, out and their strides 16-byte aligned; kv's batch stride 0, or one of its two strides a multiple of the
+ * shared_kv, out and their strides 16-byte aligned, workspace 32-byte; kv's batch stride 0, or one of its two strides a multiple of the
  * other; kv_len and shared_len at most 2^24; scale > 0. The result does not depend on timing: the same call
  * gives the same bits. Calls that may overlap on the GPU need workspaces of their own. */
 int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, const void* kv,
