@@ -40,11 +40,11 @@ int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 // Into how many parts the key lists (n tiles each) of the units that a last, partly filled round of CTAs would take
 // are cut: the parts' rounds, at 1.5 tiles of fixed cost a unit, and for any cut the merge, about 5 tiles' time
 // (a tile: 0.8 us).
-int tail_splits(int units, int n) {
+int tail_splits(int units, int n, int ctas) {
   int best = 1;
   double best_cost = n + 1.5;
   for (int k = 2; k <= 16 && n / k >= 4; ++k) {
-    const double cost = ceil_div((int64_t)units * k, kCtxRound) * (ceil_div(n, k) + 1.5) + 5;
+    const double cost = ceil_div((int64_t)units * k, ctas) * (ceil_div(n, k) + 1.5) + 5;
     if (cost < best_cost) {
       best = k;
       best_cost = cost;
@@ -70,18 +70,18 @@ Plan make_plan(const Shape& s) {
     part.use_own = own;
     part.row_tiles = ceil_div(part_rows, tiles ? 128 : p.rows_per_tile);
     const int64_t items = (int64_t)(pool ? 1 : s.B) * s.Hkv * part.row_tiles;
-    const int keys = tiles ? 128 : 2048 / s.D;
+    const int keys = tiles ? ctx_tile_keys(s.D) : 2048 / s.D, ctas = tiles ? ctx_tile_ctas(s.D) : kCtxRowCtas;
     const int chunks = (sh ? ceil_div(s.Ls, keys) : 0) + (own ? ceil_div(s.Lkv, keys) : 0);
-    // Few items: the key list is cut so that one round of CTAs fills the GPU, down to two tiles (or two chunks for
-    // each of the four warps) per CTA; the merge then costs less than the idle SMs.
-    part.splits = std::max(1, std::min({static_cast<int>(kCtxRound / items), chunks / (tiles ? 2 : 8), kMaxSplits}));
+    // Few items: the key list is cut so that one round of CTAs fills the GPU, down to 256 keys (or two chunks
+    // for each of the four warps) per CTA; the merge then costs less than the idle SMs.
+    part.splits = std::max(1, std::min({static_cast<int>(ctas / items), chunks / (tiles ? 256 / keys : 8), kMaxSplits}));
     if (tiles && s.masked) part.splits = std::max(part.splits, ceil_div(chunks, kCtxMaskTiles));
     part.count = static_cast<int>(items * part.splits);
     part.slot0 = p.slots;
     p.slots += part.splits;
-    if (tiles && !pooled && part.splits == 1 && items > kCtxRound && items % kCtxRound) {
+    if (tiles && !pooled && part.splits == 1 && items > ctas && items % ctas) {
       // Many items, and a last round that leaves CTAs idle: its items alone are cut.
-      const int tail = static_cast<int>(items % kCtxRound), k = tail_splits(tail, chunks);
+      const int tail = static_cast<int>(items % ctas), k = tail_splits(tail, chunks, ctas);
       if (k > 1) {
         CtxPart& last = p.part[1] = part;
         part.count = static_cast<int>(items - tail);

@@ -1,13 +1,14 @@
-// Context attention for many query rows: tcgen05 MMAs on 128-row x 128-key tiles.
+// Context attention for many query rows: tcgen05 MMAs on tiles of 128 rows.
 //
 // One CTA takes 128 rows of one kv head (a row: a query token and one query head of the group) and walks its keys:
-// S = Q K^T (fp32, TMEM), P = exp2(c S - m) (16-bit, TMEM), O += P V (fp32, TMEM), with the running maximum m and sum
-// of each row in the registers of one thread. The exponentials bound it (one per score against 4 D flops), and
-// one row per thread leaves each SM sub-partition a single softmax warp, which cannot fill its pipes. So two CTAs
-// share an SM, each with 256 TMEM columns. A lazy maximum (O is rescaled only when a row's maximum grows by more than
-// 2^8) keeps O in TMEM, and a quarter of the exponentials goes to the FMA pipe (exp2_poly2).
-// At D 64 P has columns of its own, so the next tile's S runs while this one's softmax does; at D 128 the columns are
-// taken (S 128, O 128), P lies over S and the other CTA fills the wait.
+// S = Q K^T (fp32, TMEM), P = exp2(c S - m) (16-bit, over S in TMEM), O += P V (fp32, TMEM), with the running maximum
+// m and sum of each row in the registers of one thread. The softmax's arithmetic bounds it: maxima, FMAs,
+// exponentials and conversions of 128 scores a row take 980 cycles of an SM with four warps on each of its
+// sub-partitions (1,170 a warp with two, 1,520 with one; measured without any memory or MMA), the MMAs of a tile 660
+// at D 64; and within a tile S, softmax and P V wait for one another, about as long again. So as many CTAs as TMEM
+// holds share an SM and fill each other's waits: at D 64 four, on tiles of 64 keys (S 64 columns, O 64), at D 128 two,
+// on tiles of 128 keys (S 128, O 128). A lazy maximum (O is rescaled only when a row's maximum grows by more than 2^8)
+// keeps O in TMEM, and a share of the exponentials goes to the FMA pipe (exp2_poly2).
 //
 // The grid is one round of CTAs; each walks its share of the units (tiles of rows), so barriers, TMEM and tensor maps
 // are set up once, K and V of the next unit are on their way early and its queries during the epilogue.
@@ -34,30 +35,32 @@ namespace hb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kLaunchRegs = 128;                 // 2 CTAs x 256 threads x 128 = the SM's 65,536
-constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
-static_assert(kSoftmaxRegs + kOtherRegs == 2 * kLaunchRegs, "the warpgroups share what the CTA was launched with");
-constexpr int kAtom = 128 * 128;                 // 128 rows of 128 bytes: 64 columns of a tile
+constexpr int kQAtom = 128 * 128;                // 128 rows of 128 bytes: 64 columns of a query tile
 constexpr float kRescaleThreshold = 8.0f;        // log2 units
-constexpr int kTmemCols = 256;
+constexpr int kCtxPolyMask = 3;                  // key pairs j with (j & 3) == 3 take exp2_poly2
 
 template <int D>
 struct Layout {
+  static constexpr int kKeys = ctx_tile_keys(D);            // of a tile
+  static constexpr int kWords = kKeys / 32;                 // of a tile's mask bits
+  static constexpr int kCtasPerSm = ctx_tile_ctas(D) / kCtxSms;
+  static constexpr int kLaunchRegs = 256 / kCtasPerSm;      // x 256 threads x kCtasPerSm = the SM's 65,536
+  static constexpr int kSoftmaxRegs = D == 64 ? 88 : 184, kOtherRegs = 2 * kLaunchRegs - kSoftmaxRegs;
+  static constexpr int kTmemCols = 512 / kCtasPerSm;        // S (and P) at 0, O at kKeys
+  static_assert(kKeys + D <= kTmemCols, "TMEM columns");
   static constexpr int kHalves = D / 64;
+  static constexpr int kAtom = kKeys * 128;                 // 64 columns of a K or V tile
   static constexpr int kTile = kHalves * kAtom;
   static constexpr int kStages = D == 64 ? 2 : 1;
-  static constexpr bool kOwnP = D == 64;                    // P beside S, not over it
-  static constexpr int kTmemP = kOwnP ? 128 : 0, kTmemO = kOwnP ? 192 : 128;  // columns; S at 0
-  static constexpr int kOffK = kTile;                       // queries at 0
+  static constexpr int kOffK = kHalves * kQAtom;            // queries at 0
   static constexpr int kOffV = kOffK + kStages * kTile;
   static constexpr int kOffBars = kOffV + kStages * kTile;
-  static constexpr int kBars = 4 * kStages + 10;
+  static constexpr int kBars = 4 * kStages + 9;
   static constexpr int kOffMisc = kOffBars + kBars * 8;     // TMEM address, abort flag
   static constexpr int kOffBits = (kOffMisc + 8 + 15) & ~15;
-  static constexpr int bytes(int mask_tiles) { return kOffBits + 2 * mask_tiles * 16 + 1024; }
+  static constexpr int bytes(int mask_tiles) { return kOffBits + 2 * mask_tiles * kWords * 4 + 1024; }
+  static_assert(kCtasPerSm * (bytes(kCtxMaskTiles) + 1024) <= 228 * 1024, "shared memory of an SM");
 };
-static_assert(Layout<64>::bytes(kCtxMaskTiles) <= 113 * 1024 && Layout<128>::bytes(kCtxMaskTiles) <= 113 * 1024,
-              "two CTAs per SM");
 
 template <bool kFp16>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
@@ -80,19 +83,43 @@ constexpr uint32_t idesc_base(bool b_mn_major) {
   const uint32_t fmt = kFp16 ? 0u : 1u;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(128 >> 4) << 24);
 }
-__device__ __forceinline__ uint32_t idesc_n(uint32_t base, int n) { return base | (static_cast<uint32_t>(n >> 3) << 17); }
+// The MMA warp runs converged, so that descriptors stay in uniform registers (inside a one-lane branch each operand of
+// each MMA is moved there one by one, which took longer than the MMAs); the elected lane's predicate picks the issuer.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_u32(bar)), "r"(lead) : "memory");
+}
 
-// Bounded waits (one second) that end early once another role has given up.
+// Bounded waits that end early once another role has given up. A try suspends the thread for a while by itself, so
+// the limit is far above any wait of a working kernel; the loop stays a few instructions long because it is inlined
+// into every hot path (a longer one, with a clock, cost the kernel its instruction cache).
+constexpr uint32_t kWaitTries = 1u << 24;
 __device__ __forceinline__ bool slow_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  const uint64_t t0 = globaltimer_ns();
-  while (!*abort_flag) {
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
-    if (globaltimer_ns() - t0 > kWaitLimitNs) {
-      record_error(HB_ERR_TIMEOUT);
-      break;
-    }
-  }
+#pragma unroll 1
+  for (uint32_t i = 0; i < kWaitTries && !*abort_flag; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  if (!*abort_flag) record_error(HB_ERR_TIMEOUT);
   *abort_flag = 1;
   return false;
 }
@@ -107,40 +134,44 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 struct Keys {
   int n0, own_len, j0, j1;
 };
+template <int kKeys>
 __device__ __forceinline__ Keys keys_of(const CtxParams& p, const CtxPart& part, const CtxUnit& u) {
   Keys k;
   k.own_len = part.use_own ? ctx_own_len(p, u.b) : 0;
-  k.n0 = part.use_shared ? (p.Ls + 127) >> 7 : 0;
-  const int n = k.n0 + ((k.own_len + 127) >> 7);
+  k.n0 = part.use_shared ? (p.Ls + kKeys - 1) / kKeys : 0;
+  const int n = k.n0 + (k.own_len + kKeys - 1) / kKeys;
   k.j0 = part.by_splits.div(u.split * n);
   k.j1 = part.by_splits.div((u.split + 1) * n);
   return k;
 }
 
-// Keys [k0, k0 + 128) of either. `hi` counts them up to the last one that may be valid (0: skip the tile); with a
+// Keys [k0, k0 + kKeys) of either. `hi` counts them up to the last one that may be valid (0: skip the tile); with a
 // mask, bits says which are.
+template <int kKeys>
 struct Tile {
   int k0, hi;
-  bool shared, full, clean;  // full: all 128 valid; clean: some of the tensor's rows in [0, hi) must not be read
-  uint4 bits;
+  bool shared, full, clean;  // full: all valid; clean: some of the tensor's rows in [0, hi) must not be read
+  uint32_t bits[kKeys / 32];
 };
-template <bool kMask>
-__device__ __forceinline__ Tile tile_of(const CtxParams& p, const Keys& ks, int j, const uint4* bits) {
-  Tile t;
+template <int kKeys, bool kMask>
+__device__ __forceinline__ Tile<kKeys> tile_of(const CtxParams& p, const Keys& ks, int j, const uint32_t* bits) {
+  Tile<kKeys> t;
   t.shared = j < ks.n0;
-  t.k0 = (t.shared ? j : j - ks.n0) * 128;
+  t.k0 = (t.shared ? j : j - ks.n0) * kKeys;
   if constexpr (kMask) {
-    t.bits = bits[j - ks.j0];
-    const uint32_t b[4] = {t.bits.x, t.bits.y, t.bits.z, t.bits.w};
     t.hi = 0;
+    uint32_t all = 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (b[i]) t.hi = 32 * i + 32 - __clz(b[i]);
-    t.full = (b[0] & b[1] & b[2] & b[3]) == 0xffffffffu;
+    for (int i = 0; i < kKeys / 32; ++i) {
+      const uint32_t b = t.bits[i] = bits[(j - ks.j0) * (kKeys / 32) + i];
+      if (b) t.hi = 32 * i + 32 - __clz(b);
+      all &= b;
+    }
+    t.full = all == 0xffffffffu;
     t.clean = !t.full;
   } else {
-    t.hi = min(128, (t.shared ? p.Ls : ks.own_len) - t.k0);
-    t.full = t.hi == 128;
+    t.hi = min(kKeys, (t.shared ? p.Ls : ks.own_len) - t.k0);
+    t.full = t.hi == kKeys;
     // rows between hi and the next multiple of 16 enter P V: zeros past the tensor, anything before its end
     t.clean = !t.shared && (t.hi & 15) && ks.own_len < p.Lkv;
   }
@@ -154,16 +185,12 @@ __device__ __forceinline__ void st_32b(void* dst, const uint32_t* v) {
                : "memory");
 }
 
-__device__ __forceinline__ uint32_t word_of(const uint4& b, int i) {
-  return i == 0 ? b.x : i == 1 ? b.y : i == 2 ? b.z : b.w;
-}
-
 template <int D, bool kFp16, bool kMask>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
     ctx_tiles_kernel(const __grid_constant__ CUtensorMap tm_own, const __grid_constant__ CUtensorMap tm_shared,
                      const __grid_constant__ CtxParams p, const int mask_tiles) {
   using L = Layout<D>;
-  constexpr int kStages = L::kStages;
+  constexpr int kStages = L::kStages, kKeys = L::kKeys, kWords = L::kWords;
   constexpr int PPR = D / 8;  // 16-byte pieces per row
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -175,15 +202,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint64_t* v_empty = v_full + kStages;     // [kStages] commit of the P V MMAs
   uint64_t* q_full = v_empty + kStages;     // 4 softmax warps wrote the queries (units that have keys)
   uint64_t* s_full = q_full + 1;            // commit: S written
-  uint64_t* s_free = s_full + 1;            // 4 softmax warps loaded S (kOwnP)
-  uint64_t* p_ready = s_free + 1;           // 4 softmax warps wrote P
-  uint64_t* o_done = p_ready + 1;           // commit: the tile's P V added
+  uint64_t* p_ready = s_full + 1;           // 4 softmax warps wrote P
+  uint64_t* o_done = p_ready + 1;           // commit: the unit's last P V added
   uint64_t* drain = o_done + 1;
   uint64_t* m_full = drain + 1;             // [2] warp 6 wrote the unit's mask bits
   uint64_t* m_free = m_full + 2;            // [2] the six roles' warps are through with them
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
-  uint4* bits0 = reinterpret_cast<uint4*>(smem + L::kOffBits);
+  uint32_t* bits0 = reinterpret_cast<uint32_t*>(smem + L::kOffBits);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count0 = p.part[0].count, total = count0 + p.part[1].count;
 
@@ -198,7 +224,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     mbar_init(q_full, 4);
     mbar_init(s_full, 1);
-    mbar_init(s_free, 4);
     mbar_init(p_ready, 4);
     mbar_init(o_done, 1);
     mbar_init(drain, 1);
@@ -210,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     fence_mbar_init();
   }
   if (warp == 5) {
-    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
   }
   // Work unit w's queries, asynchronously into the shared-memory image (rows past the end as zeros): warp i its 32
@@ -222,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const CtxUnit u = ctx_unit(p, part, w - (w >= count0 ? count0 : 0));
     const bool plain = p.G == 1 && !part.pooled;  // rows one stride apart
     const uint16_t* src = p.q + (plain ? u.b * p.q_bs + (int64_t)(u.rt * 128 + qrow) * p.q_rs + u.g * D : 0) + qch * 8;
-    const uint32_t dst = smem_u32(smem) + (qch >> 3) * kAtom;
+    const uint32_t dst = smem_u32(smem) + (qch >> 3) * kQAtom;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       const int lr = qrow + i * kRowsPerStep, r = u.rt * 128 + lr;
@@ -244,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegs));
     if (warp == 4 && lane == 0) {
       // -------------------------------------------------------------- TMA producer
       int it = 0;
@@ -252,12 +277,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int n = 0, w = blockIdx.x; ok && w < total; ++n, w += gridDim.x) {
         const CtxPart& part = p.part[w >= count0 ? 1 : 0];
         const CtxUnit u = ctx_unit(p, part, w - (w >= count0 ? count0 : 0));
-        const Keys ks = keys_of(p, part, u);
-        const uint4* bits = bits0 + (n & 1) * mask_tiles;
+        const Keys ks = keys_of<kKeys>(p, part, u);
+        const uint32_t* bits = bits0 + (n & 1) * mask_tiles * kWords;
         const int kcol = u.g * D, vcol = p.Hkv * D + u.g * D;
         if (kMask && !(ok = role_wait(&m_full[n & 1], (n >> 1) & 1, abort_flag))) break;
         for (int j = ks.j0; j < ks.j1; ++j) {
-          const Tile t = tile_of<kMask>(p, ks, j, bits);
+          const Tile<kKeys> t = tile_of<kKeys, kMask>(p, ks, j, bits);
           if (t.hi <= 0) continue;
           const int st = it % kStages;
           const uint32_t ph = ((it / kStages) & 1) ^ 1;
@@ -269,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           mbar_arrive_expect_tx(&k_full[st], L::kTile);
 #pragma unroll
           for (int h = 0; h < L::kHalves; ++h)
-            tma_load_3d(smem + L::kOffK + st * L::kTile + h * kAtom, tm, kcol + 64 * h, c1, c2, &k_full[st]);
+            tma_load_3d(smem + L::kOffK + st * L::kTile + h * L::kAtom, tm, kcol + 64 * h, c1, c2, &k_full[st]);
           if (it >= kStages && !(ok = role_wait(&v_empty[st], ph, abort_flag))) {
             mbar_wait(&k_full[st], (it / kStages) & 1);  // K was issued already
             break;
@@ -277,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           mbar_arrive_expect_tx(&v_full[st], L::kTile);
 #pragma unroll
           for (int h = 0; h < L::kHalves; ++h)
-            tma_load_3d(smem + L::kOffV + st * L::kTile + h * kAtom, tm, vcol + 64 * h, c1, c2, &v_full[st]);
+            tma_load_3d(smem + L::kOffV + st * L::kTile + h * L::kAtom, tm, vcol + 64 * h, c1, c2, &v_full[st]);
           ++it;
         }
         if (kMask) mbar_arrive(&m_free[n & 1]);
@@ -287,40 +312,40 @@ __global__ void __launch_bounds__(kThreads, 2)
         mbar_wait(&k_full[i % kStages], (i / kStages) & 1);
         mbar_wait(&v_full[i % kStages], (i / kStages) & 1);
       }
-    } else if (warp == 5 && lane == 0) {
+    } else if (warp == 5) {
+      const uint32_t lead = elect_one();
       // -------------------------------------------------------------- MMA issuer
       constexpr uint32_t idS = idesc_base<kFp16>(false), idO = idesc_base<kFp16>(true) | ((D >> 3) << 17);
       const uint64_t dq = smem_desc_sw128(smem_u32(smem));
       const uint64_t dk = smem_desc_sw128(smem_u32(smem + L::kOffK));
       // V tiles are MN-major: 16 keys are 2,048 bytes on, the second 64 columns one atom on
-      const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kOffV), D == 64 ? 16 : kAtom);
-      const uint32_t tS = tmem, tP = tmem + L::kTmemP, tO = tmem + L::kTmemO;
+      const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kOffV), D == 64 ? 16 : L::kAtom);
+      const uint32_t tS = tmem, tO = tmem + kKeys;
       int it = 0, units = 0;
       auto issue_s = [&](int i, int n16) {
         const int st = i % kStages;
-        if (L::kOwnP && i > 0 && !role_wait(s_free, (i - 1) & 1, abort_flag)) return false;
-        if (!role_wait(&k_full[st], (i / kStages) & 1, abort_flag)) return false;
+        if (!warp_wait(&k_full[st], (i / kStages) & 1, abort_flag)) return false;
         tc_fence_after();
         const uint32_t id = idS | (static_cast<uint32_t>(n16 >> 3) << 17);
         const uint64_t kd = dk + st * (L::kTile >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = ((k / 4) * kAtom + (k % 4) * 32) >> 4;
-          mma_bf16_ss(tS, dq + off, kd + off, id, k > 0);
+          const int half = k / 4, at = (k % 4) * 32;
+          mma_ss(lead, tS, dq + ((half * kQAtom + at) >> 4), kd + ((half * L::kAtom + at) >> 4), id, k > 0);
         }
-        tc_commit(s_full);
-        tc_commit(&k_empty[st]);
+        commit(lead, s_full);
+        commit(lead, &k_empty[st]);
         return true;
       };
       bool ok = true;
       for (int n = 0, w = blockIdx.x; ok && w < total; ++n, w += gridDim.x) {
         const CtxPart& part = p.part[w >= count0 ? 1 : 0];
-        const Keys ks = keys_of(p, part, ctx_unit(p, part, w - (w >= count0 ? count0 : 0)));
-        const uint4* bits = bits0 + (n & 1) * mask_tiles;
-        if (kMask && !(ok = role_wait(&m_full[n & 1], (n >> 1) & 1, abort_flag))) break;
+        const Keys ks = keys_of<kKeys>(p, part, ctx_unit(p, part, w - (w >= count0 ? count0 : 0)));
+        const uint32_t* bits = bits0 + (n & 1) * mask_tiles * kWords;
+        if (kMask && !(ok = warp_wait(&m_full[n & 1], (n >> 1) & 1, abort_flag))) break;
         auto next_tile = [&](int j, int& n16) {  // the first tile at or after j that has valid keys
           for (; j < ks.j1; ++j) {
-            const Tile t = tile_of<kMask>(p, ks, j, bits);
+            const Tile<kKeys> t = tile_of<kKeys, kMask>(p, ks, j, bits);
             n16 = (t.hi + 15) & ~15;
             if (t.hi > 0) break;
           }
@@ -328,67 +353,67 @@ __global__ void __launch_bounds__(kThreads, 2)
         };
         int n16 = 0, n16_next = 0;
         int j = next_tile(ks.j0, n16);
-        if (j < ks.j1) ok = role_wait(q_full, units++ & 1, abort_flag) && issue_s(it, n16);
+        if (j < ks.j1) ok = warp_wait(q_full, units++ & 1, abort_flag) && issue_s(it, n16);
         for (bool first = true; ok && j < ks.j1; first = false) {
           const int jn = next_tile(j + 1, n16_next), st = it % kStages;
-          // P beside S: the next S while the softmax computes this tile's P
-          if (L::kOwnP && jn < ks.j1 && !(ok = issue_s(it + 1, n16_next))) break;
-          if (!(ok = role_wait(&v_full[st], (it / kStages) & 1, abort_flag) && role_wait(p_ready, it & 1, abort_flag)))
+          if (!(ok = warp_wait(&v_full[st], (it / kStages) & 1, abort_flag) && warp_wait(p_ready, it & 1, abort_flag)))
             break;
           tc_fence_after();
           const uint64_t vd = dv + st * (L::kTile >> 4);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (16 * k < n16) mma_bf16_ts(tO, tP + 8 * k, vd + k * (2048 >> 4), idO, !first || k > 0);
-          tc_commit(o_done);
-          tc_commit(&v_empty[st]);
-          // P over S: in the tensor pipe's order, P V reads P before the next S overwrites it
-          if (!L::kOwnP && jn < ks.j1 && !(ok = issue_s(it + 1, n16_next))) break;
+          for (int k = 0; k < kKeys / 16; ++k)
+            if (16 * k < n16) mma_ts(lead, tO, tS + 8 * k, vd + k * (2048 >> 4), idO, !first || k > 0);
+          if (jn >= ks.j1) commit(lead, o_done);
+          commit(lead, &v_empty[st]);
+          // in the tensor pipe's order: P V reads P before the next S overwrites it
+          if (jn < ks.j1 && !(ok = issue_s(it + 1, n16_next))) break;
           ++it;
           j = jn;
           n16 = n16_next;
         }
-        if (kMask) mbar_arrive(&m_free[n & 1]);
+        if (kMask && lead) mbar_arrive(&m_free[n & 1]);
       }
-      tc_commit(drain);  // every MMA this thread issued has finished before TMEM is freed
+      commit(lead, drain);  // every MMA this thread issued has finished before TMEM is freed
       mbar_wait(drain, 0);
     } else if (kMask && warp == 6) {
       // -------------------------------------------------------------- mask bits, one unit ahead of their readers
       for (int n = 0, w = blockIdx.x; w < total; ++n, w += gridDim.x) {
         const CtxPart& part = p.part[w >= count0 ? 1 : 0];
         const CtxUnit u = ctx_unit(p, part, w - (w >= count0 ? count0 : 0));
-        const Keys ks = keys_of(p, part, u);
-        uint4* bits = bits0 + (n & 1) * mask_tiles;
+        const Keys ks = keys_of<kKeys>(p, part, u);
+        uint32_t* bits = bits0 + (n & 1) * mask_tiles * kWords;
         if (n >= 2 && !warp_wait(&m_free[n & 1], ((n >> 1) & 1) ^ 1, abort_flag)) break;
         for (int j = ks.j0; j < ks.j1; ++j) {
           const bool sh = j < ks.n0;
-          const int k0 = (sh ? j : j - ks.n0) * 128, len = sh ? p.Ls : ks.own_len;
+          const int k0 = (sh ? j : j - ks.n0) * kKeys, len = sh ? p.Ls : ks.own_len;
           const uint8_t* mk = sh ? p.smask : (p.mask ? p.mask + u.b * p.mask_bs : nullptr);
-          uint32_t v[4];
+          uint32_t v[kWords];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < kWords; ++i) {
             const int k = k0 + 32 * i + lane;
             v[i] = k < len ? (mk ? mk[k] : 1u) : 0u;
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = __ballot_sync(0xffffffffu, v[i] != 0u);
-          if (lane == 0) bits[j - ks.j0] = make_uint4(v[0], v[1], v[2], v[3]);
+          for (int i = 0; i < kWords; ++i) {
+            v[i] = __ballot_sync(0xffffffffu, v[i] != 0u);
+            if (lane == 0) bits[(j - ks.j0) * kWords + i] = v[i];
+          }
         }
         if (lane == 0) mbar_arrive(&m_full[n & 1]);  // lane 0 wrote them all
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));
     const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t tS = tmem + lane_base, tP = tS + L::kTmemP, tO = tS + L::kTmemO;
+    const uint32_t tS = tmem + lane_base, tO = tS + kKeys;
     const int row = warp * 32 + lane;
-    int it = 0;
+    int it = 0, done = 0;
     bool ok = true;
     for (int n = 0, w = blockIdx.x; ok && w < total; ++n, w += gridDim.x) {
       const CtxPart& part = p.part[w >= count0 ? 1 : 0];
       const CtxUnit u = ctx_unit(p, part, w - (w >= count0 ? count0 : 0));
-      const Keys ks = keys_of(p, part, u);
-      const uint4* bits = bits0 + (n & 1) * mask_tiles;
+      const Keys ks = keys_of<kKeys>(p, part, u);
+      const uint32_t* bits = bits0 + (n & 1) * mask_tiles * kWords;
       if (kMask && !(ok = warp_wait(&m_full[n & 1], (n >> 1) & 1, abort_flag))) break;
       // -------------------------------------------------------------- queries: each lane's own pieces have landed
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -398,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int e = 0; e < 8; ++e) wv[e] = __ldg(p.q_w + qch * 8 + e);
 #pragma unroll 2
         for (int i = 0; i < kSteps; ++i) {
-          uint4* at = reinterpret_cast<uint4*>(smem + (qch >> 3) * kAtom + sw128_offset(qrow + i * kRowsPerStep, qch & 7));
+          uint4* at = reinterpret_cast<uint4*>(smem + (qch >> 3) * kQAtom + sw128_offset(qrow + i * kRowsPerStep, qch & 7));
           const uint4 v = *at;
           uint32_t x[4] = {v.x, v.y, v.z, v.w};
           float2 f[4];
@@ -423,26 +448,21 @@ __global__ void __launch_bounds__(kThreads, 2)
       float m = -INFINITY, l = 0.f;
       bool first = true;
       for (int j = ks.j0; j < ks.j1; ++j) {
-        const Tile t = tile_of<kMask>(p, ks, j, bits);
+        const Tile<kKeys> t = tile_of<kKeys, kMask>(p, ks, j, bits);
         if (t.hi <= 0) continue;
         if (first && lane == 0) mbar_arrive(q_full);
         if (!(ok = warp_wait(s_full, it & 1, abort_flag))) break;
         tc_fence_after();
-        uint32_t r[4][32];
+        uint32_t r[kWords][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, r[c]);
+        for (int c = 0; c < kWords; ++c) tmem_ld32(tS + 32 * c, r[c]);
         tmem_wait_ld();
-        if constexpr (L::kOwnP) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_free);
-        }
         if (!t.full) {  // columns past hi hold an earlier tile's bits
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < kWords; ++c) {
             uint32_t word;
             if constexpr (kMask) {
-              word = word_of(t.bits, c);
+              word = t.bits[c];
             } else {
               const int left = t.hi - 32 * c;
               word = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
@@ -454,10 +474,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < kWords; ++c)
 #pragma unroll
           for (int e = 0; e < 32; e += 2)
-            mx[c] = fmax3(mx[c], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+            mx[e / 2 & 3] = fmax3(mx[e / 2 & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
         const float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
         const float m_new = fmaxf(m, rmax);
         const bool upd = m_new > m + kRescaleThreshold;
@@ -468,17 +488,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         const float nm = m == -INFINITY ? 0.f : -m;
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
-        // the tile before's P V has read P and written O
-        if (!first && !(ok = warp_wait(o_done, (it - 1) & 1, abort_flag))) break;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < kWords; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float x0, x1, p0, p1;
             ffma2(x0, x1, __uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1]), p.scale_log2, p.scale_log2,
                   nm, nm);
-            if ((e & kPolyMask) == kPolyMask) {  // a share of the exponentials on the FMA pipe
+            if ((e & kCtxPolyMask) == kCtxPolyMask) {  // a share of the exponentials on the FMA pipe
               exp2_poly2(x0, x1, p0, p1);
             } else {
               p0 = ex2_approx(x0);
@@ -489,11 +507,10 @@ __global__ void __launch_bounds__(kThreads, 2)
             // P in the input's type for the MMA (at most 2^8 above 1, relative error up to 2^-8 or 2^-11)
             pk[e] = pack16<kFp16>(p0, p1);
           }
-          tmem_st16(tP + 16 * c, pk);
+          tmem_st16(tS + 16 * c, pk);
         }
         l = l * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
-        if (!first && __any_sync(0xffffffffu, upd)) {
-          tc_fence_after();
+        if (!first && __any_sync(0xffffffffu, upd)) {  // (S of this tile came after the last one's P V)
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -504,16 +521,25 @@ __global__ void __launch_bounds__(kThreads, 2)
             tmem_st32(tO + 32 * c, o);
           }
         }
-        if (t.clean) {  // this thread's V row, where its key is not valid
+        if (t.clean) {  // V rows of keys that are not valid: 128 / kKeys threads to a row
           const int st = it % kStages;
           if (!(ok = warp_wait(&v_full[st], (it / kStages) & 1, abort_flag))) break;
-          bool valid = row < t.hi;
-          if constexpr (kMask) valid = (word_of(t.bits, warp) >> lane) & 1u;
+          const int key = row % kKeys;
+          bool valid = key < t.hi;
+          if constexpr (kMask) {
+            valid = false;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+              if (key / 32 == i) valid = (t.bits[i] >> lane) & 1u;
+          }
           if (!valid) {
+            constexpr int kPieces = PPR * kKeys / 128;
             uint8_t* v = smem + L::kOffV + st * L::kTile;
 #pragma unroll
-            for (int c = 0; c < PPR; ++c)
-              *reinterpret_cast<uint4*>(v + (c >> 3) * kAtom + sw128_offset(row, c & 7)) = make_uint4(0u, 0u, 0u, 0u);
+            for (int c = 0; c < kPieces; ++c) {
+              const int ch = row / kKeys * kPieces + c;
+              *reinterpret_cast<uint4*>(v + (ch >> 3) * L::kAtom + sw128_offset(key, ch & 7)) = make_uint4(0u, 0u, 0u, 0u);
+            }
           }
           fence_proxy_async_smem();
         }
@@ -528,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       // -------------------------------------------------------------- epilogue: one row per thread
       if (!ok) break;
       if (w + gridDim.x < total) load_q(w + gridDim.x);  // (the S MMAs of this unit are done)
-      if (!first && !(ok = warp_wait(o_done, (it - 1) & 1, abort_flag))) break;
+      if (!first && !(ok = warp_wait(o_done, done++ & 1, abort_flag))) break;
       tc_fence_after();
       const int gr = u.rt * 128 + row;
       const bool live = gr < u.rows;
@@ -579,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   if (warp == 5) {
     tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    tmem_dealloc(tmem, L::kTmemCols);
   }
 }
 
@@ -595,15 +621,15 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// `outer` x `mid` rows of `width` states; box 64 columns x 128 keys (the middle dimension, or the outer one where
+// `outer` x `mid` rows of `width` states; box 64 columns x `keys` keys (the middle dimension, or the outer one where
 // `keys_outer`), 128-byte swizzle; keys past the end read as zero.
-bool encode_states(CUtensorMap* map, const void* base, bool fp16, int64_t width, int64_t mid, int64_t outer,
-                   int64_t mid_stride, int64_t outer_stride, bool keys_outer) {
+bool encode_states(CUtensorMap* map, const void* base, bool fp16, unsigned keys, int64_t width, int64_t mid,
+                   int64_t outer, int64_t mid_stride, int64_t outer_stride, bool keys_outer) {
   auto encode = encode_fn();
   if (!encode) return false;
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(mid), static_cast<cuuint64_t>(outer)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(mid_stride) * 2, static_cast<cuuint64_t>(outer_stride) * 2};
-  cuuint32_t box[3] = {64, keys_outer ? 1u : 128u, keys_outer ? 128u : 1u};
+  cuuint32_t box[3] = {64, keys_outer ? 1u : keys, keys_outer ? keys : 1u};
   cuuint32_t estr[3] = {1, 1, 1};
   return encode(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
                 const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -615,14 +641,14 @@ template <int D, bool kFp16, bool kMask>
 int launch_tiles(const CUtensorMap& own, const CUtensorMap& shared, const CtxParams& p, int mask_tiles,
                  cudaStream_t s) {
   auto kernel = ctx_tiles_kernel<D, kFp16, kMask>;
-  // setmaxnreg's split counts on exactly kLaunchRegs registers per thread at launch (an increase that the CTA's
-  // registers do not cover would never be granted), and two CTAs per SM on their TMEM
+  // setmaxnreg's split counts on exactly kLaunchRegs registers per thread at launch: an increase that the CTA's
+  // registers do not cover would never be granted
   cudaFuncAttributes attr{};
-  if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess || attr.numRegs != kLaunchRegs) return HB_ERR_LAUNCH;
+  if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess || attr.numRegs != Layout<D>::kLaunchRegs) return HB_ERR_LAUNCH;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::bytes(kCtxMaskTiles)) !=
       cudaSuccess)
     return HB_ERR_LAUNCH;
-  const int grid = std::min(p.part[0].count + p.part[1].count, kCtxRound);
+  const int grid = std::min(p.part[0].count + p.part[1].count, ctx_tile_ctas(D));
   kernel<<<grid, kThreads, Layout<D>::bytes(mask_tiles), s>>>(own, shared, p, mask_tiles);
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
@@ -646,16 +672,17 @@ int ctx_tiles_take_status(unsigned int* status) {
 
 int launch_ctx_tiles(const CtxParams& p, int D, bool fp16, int mask_tiles, cudaStream_t s) {
   const int64_t width = 2ll * p.Hkv * D;
+  const unsigned keys = ctx_tile_keys(D);
   CUtensorMap own{}, shared{};
   const bool use_own = p.Lkv > 0 && (p.part[0].use_own || p.part[1].use_own);
   const bool use_shared = p.part[0].use_shared != 0;
   const int64_t batch = p.kv_bs == 0 ? 1 : p.B;  // one copy of the states is a batch of one to the map
   if (use_own &&
-      !(p.kv_inter ? encode_states(&own, p.kv, fp16, width, batch, p.Lkv, p.kv_bs, p.kv_rs, true)
-                   : encode_states(&own, p.kv, fp16, width, p.Lkv, batch, p.kv_rs,
+      !(p.kv_inter ? encode_states(&own, p.kv, fp16, keys, width, batch, p.Lkv, p.kv_bs, p.kv_rs, true)
+                   : encode_states(&own, p.kv, fp16, keys, width, p.Lkv, batch, p.kv_rs,
                                    batch > 1 ? p.kv_bs : p.kv_rs * p.Lkv, false)))
     return HB_ERR_LAUNCH;
-  if (use_shared && !encode_states(&shared, p.skv, fp16, width, p.Ls, 1, p.skv_rs, p.skv_rs * p.Ls, false))
+  if (use_shared && !encode_states(&shared, p.skv, fp16, keys, width, p.Ls, 1, p.skv_rs, p.skv_rs * p.Ls, false))
     return HB_ERR_LAUNCH;
   if (!use_own) own = shared;
   if (!use_shared) shared = own;
