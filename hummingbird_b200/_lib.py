@@ -32,8 +32,7 @@ SIGNATURES: dict[str, list] = {
                                    _f, _i, _i, _p],
     "hb_cross_diff_attn": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _f, _p],
     "hb_context_workspace_bytes": [_i, _i, _i, _i, _i, _i, _i, _i, C.POINTER(_sz)],
-    "hb_context_attn": [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _p, _p, _f, _f, _p, _i64, _i64, _i, _i,
-                        _i, _i, _i, _i, _i, _i, _p, _sz, _p],
+    "hb_context_attn": [C.c_char_p, _p],  # HbContextArgs, packed by context_attention
     "hb_band_workspace_bytes": [_i, _i, _i, _i, _i, C.POINTER(_sz)],
     "hb_band_diff_attn": [_p, _i64, _p, _p, _p, _i, _p, _p, _i64, _i, _i, _i, _i, _i64, _i, _i, _i, _i, _i, _p, _sz,
                           _i, _p],
@@ -76,7 +75,11 @@ def lib() -> C.CDLL:
 
 def call(name: str, *args) -> None:
     """Call an entry point; HB_ERR_SHAPE becomes ValueError (as the reference raises), others HbError."""
-    code = getattr(lib(), name)(*args)
+    check(name, getattr(lib(), name)(*args))
+
+
+def check(name: str, code: int) -> None:
+    """Raise for an entry point's status, as `call` does."""
     if code == HB_ERR_SHAPE:
         raise ValueError(f"{name}: unsupported shape or argument")
     if code != HB_OK:

@@ -3,6 +3,8 @@ from __future__ import annotations
 
 import torch
 
+from hummingbird_b200 import _lib
+
 
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
@@ -16,6 +18,25 @@ def check_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if not t.is_cuda:
             raise RuntimeError("hummingbird_b200 operators run on CUDA tensors only (there is no CPU path)")
+
+
+try:  # the current stream's handle without building a torch.cuda.Stream around it (2 us)
+    from torch._C import _cuda_getCurrentRawStream as raw_stream
+except ImportError:
+    def raw_stream(device: int) -> int:
+        return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch_on(device: int, name: str, fn, *args) -> None:
+    """Call entry point `fn` with its arguments and the current stream of CUDA device `device`, with that device
+    current."""
+    if torch.cuda.current_device() == device:
+        code = fn(*args, raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, raw_stream(device))
+    if code:
+        _lib.check(name, code)
 
 
 _WS: dict[int, torch.Tensor] = {}

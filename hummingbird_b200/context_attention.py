@@ -13,107 +13,131 @@ Inference only: tensors that require gradients are refused. `ValueError` on unsu
 from __future__ import annotations
 
 import ctypes
-import functools
+import struct
 
 import torch
 
 from hummingbird_b200 import _lib
-from hummingbird_b200._tensors import check_cuda
+from hummingbird_b200._tensors import check_cuda, launch_on
 
 _DTYPES = {torch.bfloat16: _lib.HB_BF16, torch.float16: _lib.HB_FP16}
+_ARGS = struct.Struct("=9Q9q8i2f")  # HbContextArgs: pointers, strides, sizes, eps and scale
+_PLANS: dict = {}                   # checked calls by the sizes, strides and types of their tensors
+_MAX_PLANS = 4096
 
 
-@functools.lru_cache(maxsize=4096)
-def _workspace_bytes(*sizes: int) -> int:
-    n = ctypes.c_size_t(0)
-    _lib.call("hb_context_workspace_bytes", *sizes, ctypes.byref(n))
-    return n.value
+def _layout(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
 
 
-def _rows(t: torch.Tensor, name: str, width: int, dtype: torch.dtype, device: torch.device,
-          batch: int | None) -> torch.Tensor:
-    """`t` checked, and copied only where the kernels cannot read its layout (unit stride in the last dim, other
-    strides multiples of 16 bytes, no row over another)."""
-    if t.dim() != (2 if batch is None else 3) or t.shape[-1] != width or (batch is not None and t.shape[0] != batch):
-        raise ValueError(f"{name} must be {'(Ls' if batch is None else '(B, Lkv'}, {width}), got {tuple(t.shape)}")
-    if t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
-    return _readable(t, width)
+def _readable(t: torch.Tensor, width: int) -> bool:
+    """Whether a tensor map describes the rows of `t`: unit stride in the last dim, the others multiples of 16 bytes,
+    no row over another, batch elements behind one another, interleaved or all the same."""
+    *outer, row, col = t.stride()
+    if col != 1 or row < width or row % 8:
+        return False
+    return not outer or outer[0] == 0 or (outer[0] >= width and outer[0] % 8 == 0
+                                          and (outer[0] % row == 0 or row % outer[0] == 0))
 
 
-def _readable(t: torch.Tensor, width: int) -> torch.Tensor:
-    """`t`, or a copy of it where a tensor map cannot describe its rows."""
-    strides = t.stride()
-    if strides[-1] == 1 and t.data_ptr() % 16 == 0 and strides[-2] >= width and strides[-2] % 8 == 0:
-        if t.dim() == 2:
-            return t
-        row, batch = strides[1], strides[0]
-        if batch == 0 or (batch >= width and batch % 8 == 0 and (batch % row == 0 or row % batch == 0)):
-            return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
-
-
-def _byte_mask(t: torch.Tensor | None, name: str, shape: tuple, device: torch.device) -> torch.Tensor | None:
-    if t is None:
-        return None
-    if t.dtype not in (torch.bool, torch.uint8) or tuple(t.shape) != shape or t.device != device:
-        raise ValueError(f"{name} must be a bool {shape} tensor on {device}, got {tuple(t.shape)} {t.dtype}")
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
-
-
-def _attend(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_mask, q_weight, eps, scale, out):
-    kv_heads = num_heads if kv_heads is None else kv_heads
+def _plan(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_mask, q_weight, out):
+    """Check a call by its sizes and types: (tensors that need a copy, workspace bytes, sizes for HbContextArgs)."""
     if head_dim not in (64, 128) or num_heads < 1 or kv_heads < 1 or num_heads % kv_heads:
         raise ValueError(f"context attention takes head_dim 64 or 128 and num_heads a multiple of kv_heads, got "
                          f"head_dim={head_dim}, {num_heads} heads, {kv_heads} kv heads")
-    width, dtype, device = num_heads * head_dim, q.dtype, q.device
+    width, kv_width, dtype = num_heads * head_dim, 2 * kv_heads * head_dim, q.dtype
     if q.dim() != 3 or dtype not in _DTYPES or q.shape[-1] != width:
         raise ValueError(f"q must be bf16 or fp16 (B, Lq, {width}), got {tuple(q.shape)} {dtype}")
     batch, q_len, _ = q.shape
-    kv = _rows(kv, "kv", 2 * kv_heads * head_dim, dtype, device, batch)
-    kv_len = kv.shape[1]
-    shared_len = 0
+    if kv.dim() != 3 or kv.shape[0] != batch or kv.shape[-1] != kv_width or kv.dtype != dtype:
+        raise ValueError(f"kv must be {dtype} ({batch}, Lkv, {kv_width}), got {tuple(kv.shape)} {kv.dtype}")
+    kv_len, shared_len = kv.shape[1], 0
     if shared_kv is not None:
-        shared_kv = _rows(shared_kv, "shared_kv", 2 * kv_heads * head_dim, dtype, device, None)
+        if shared_kv.dim() != 2 or shared_kv.shape[-1] != kv_width or shared_kv.dtype != dtype:
+            raise ValueError(f"shared_kv must be {dtype} (Ls, {kv_width}), got {tuple(shared_kv.shape)} "
+                             f"{shared_kv.dtype}")
         shared_len = shared_kv.shape[0]
-    if lens is not None and (lens.dtype != torch.int32 or tuple(lens.shape) != (batch,) or lens.device != device):
-        raise ValueError(f"lens must be int32 ({batch},) on {device}, got {tuple(lens.shape)} {lens.dtype}")
-    mask = _byte_mask(mask, "mask", (batch, kv_len), device)
-    shared_mask = _byte_mask(shared_mask, "shared_mask", (shared_len,), device)
-    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.device != device
-                            or out.stride(-1) != 1):
-        raise ValueError(f"out must be {dtype} {tuple(q.shape)} on {device} with unit stride in its last dim")
-    check_cuda(q)
-    if torch.is_grad_enabled() and (q.requires_grad or kv.requires_grad
-                                    or (shared_kv is not None and shared_kv.requires_grad)):
+    if lens is not None and (lens.dtype != torch.int32 or lens.shape != (batch,)):
+        raise ValueError(f"lens must be int32 ({batch},), got {tuple(lens.shape)} {lens.dtype}")
+    for name, t, shape in (("mask", mask, (batch, kv_len)), ("shared_mask", shared_mask, (shared_len,))):
+        if t is not None and (t.dtype not in (torch.bool, torch.uint8) or t.shape != shape):
+            raise ValueError(f"{name} must be bool {shape}, got {tuple(t.shape)} {t.dtype}")
+    if q_weight is not None and q_weight.shape != (head_dim,):
+        raise ValueError(f"q_weight must be ({head_dim},), got {tuple(q_weight.shape)}")
+    if out is not None and (out.shape != q.shape or out.dtype != dtype or out.stride(-1) != 1):
+        raise ValueError(f"out must be {dtype} {tuple(q.shape)} with unit stride in its last dim")
+    check_cuda(*(t for t in (q, kv, shared_kv, lens, mask, shared_mask, q_weight, out) if t is not None))
+    copies = (not _readable(q, width), not _readable(kv, kv_width),
+              shared_kv is not None and not _readable(shared_kv, kv_width),
+              lens is not None and lens.stride(0) != 1,
+              mask is not None and kv_len > 1 and mask.stride(1) != 1,
+              shared_mask is not None and shared_len > 1 and shared_mask.stride(0) != 1,
+              q_weight is not None and (q_weight.dtype != torch.float32 or q_weight.stride(0) != 1))
+    need = 0
+    if batch and q_len:
+        n = ctypes.c_size_t(0)
+        _lib.call("hb_context_workspace_bytes", batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim,
+                  int(mask is not None or shared_mask is not None), ctypes.byref(n))
+        need = n.value
+    strides = (q.stride(0), q.stride(1), kv.stride(0), kv.stride(1), 0 if shared_kv is None else shared_kv.stride(0),
+               0 if mask is None else mask.stride(0))
+    sizes = (batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim, _DTYPES[dtype])
+    return any(copies) and copies, need, strides, sizes, q.is_contiguous() and batch * q_len > 0
+
+
+def _own_copy(t: torch.Tensor, copy: bool, dtype=None):
+    return t.to(dtype or t.dtype, copy=True, memory_format=torch.contiguous_format) if copy else t
+
+
+def _attend(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_mask, q_weight, eps, scale, out):
+    if kv_heads is None:
+        kv_heads = num_heads
+    key = (num_heads, head_dim, kv_heads, q.shape, q.stride(), q.dtype, kv.shape, kv.stride(), kv.dtype,
+           _layout(shared_kv), _layout(lens), _layout(mask), _layout(shared_mask), _layout(q_weight), _layout(out))
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _plan(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_mask, q_weight, out)
+        if len(_PLANS) >= _MAX_PLANS:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    copies, need, strides, sizes, like_q = plan
+    device = q.get_device()
+    for t in (kv, shared_kv, lens, mask, shared_mask, q_weight, out):
+        if t is not None and t.get_device() != device:
+            check_cuda(q, t)
+            raise ValueError("the tensors of a context attention must be on one device")
+    if device < 0:
+        check_cuda(q)
+    if (q.requires_grad or kv.requires_grad or (shared_kv is not None and shared_kv.requires_grad)) \
+            and torch.is_grad_enabled():
         raise RuntimeError("context attention has no backward pass: call it under torch.no_grad()")
-    q = _readable(q, width)
-    if lens is not None and lens.stride(0) != 1:
-        lens = lens.contiguous()
-    if q_weight is not None:
-        if tuple(q_weight.shape) != (head_dim,) or q_weight.device != device:
-            raise ValueError(f"q_weight must be ({head_dim},) on {device}, got {tuple(q_weight.shape)}")
-        q_weight = q_weight.to(torch.float32).contiguous()
-        if q_weight.data_ptr() % 16:
-            q_weight = q_weight.clone()
+    q_at, kv_at = q.data_ptr(), kv.data_ptr()
+    shared_at = 0 if shared_kv is None else shared_kv.data_ptr()
+    weight_at = 0 if q_weight is None else q_weight.data_ptr()
+    if copies or (q_at | kv_at | shared_at | weight_at) & 15:
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        c = copies or (False,) * 7
+        return _attend(_own_copy(q, c[0] or q_at & 15), shared_kv if shared_kv is None else
+                       _own_copy(shared_kv, c[2] or shared_at & 15), _own_copy(kv, c[1] or kv_at & 15), num_heads,
+                       head_dim, kv_heads, lens if lens is None else _own_copy(lens, c[3]),
+                       mask if mask is None else _own_copy(mask, c[4]),
+                       shared_mask if shared_mask is None else _own_copy(shared_mask, c[5]),
+                       q_weight if q_weight is None else _own_copy(q_weight, c[6] or weight_at & 15, torch.float32),
+                       eps, scale, out)
     if out is None:
-        out = torch.empty(batch, q_len, width, dtype=dtype, device=device)
-    if not batch or not q_len:
+        out = torch.empty_like(q) if like_q else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if not sizes[0] or not sizes[1]:
         return out
-    need = _workspace_bytes(batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim,
-                            int(mask is not None or shared_mask is not None))
-    # partial results in a block of the caching allocator: it belongs to this call's stream, or to the graph that
-    # is being captured, so calls on other streams and other graphs have theirs
-    with torch.cuda.device(device):
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        _lib.call("hb_context_attn", q.data_ptr(), q.stride(0), q.stride(1), kv.data_ptr(), kv.stride(0), kv.stride(1),
-                  None if shared_kv is None else shared_kv.data_ptr(), 0 if shared_kv is None else shared_kv.stride(0),
-                  None if lens is None else lens.data_ptr(), None if mask is None else mask.data_ptr(),
-                  0 if mask is None else mask.stride(0), None if shared_mask is None else shared_mask.data_ptr(),
-                  None if q_weight is None else q_weight.data_ptr(), eps,
-                  head_dim ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0), out.stride(1), batch,
-                  q_len, kv_len, shared_len, num_heads, kv_heads, head_dim, _DTYPES[dtype],
-                  None if ws is None else ws.data_ptr(), need, torch.cuda.current_stream(device).cuda_stream)
+    # Partial results in a block of the caching allocator: it belongs to this call's stream, or to the graph that is
+    # being captured, so calls on other streams and other graphs have theirs.
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    out_strides = out.stride()
+    args = _ARGS.pack(q_at, kv_at, shared_at, 0 if lens is None else lens.data_ptr(),
+                      0 if mask is None else mask.data_ptr(), 0 if shared_mask is None else shared_mask.data_ptr(),
+                      weight_at, out.data_ptr(), 0 if ws is None else ws.data_ptr(), *strides, out_strides[0],
+                      out_strides[1], need, *sizes, eps, head_dim ** -0.5 if scale is None else scale)
+    launch_on(device, "hb_context_attn", _lib.lib().hb_context_attn, args)
     return out
 
 

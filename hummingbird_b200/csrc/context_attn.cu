@@ -58,8 +58,9 @@ Plan make_plan(const Shape& s) {
   const int G = s.H / s.Hkv;
   const int rows = s.Lq * G;
   // One pass over the shared keys for all batch elements pays where an element's rows would leave most of a
-  // 128-row tile empty; otherwise each element walks them in the same pass as its own.
-  const bool pooled = s.Ls > 0 && s.B > 1 && rows < 128;
+  // 128-row tile empty and the passes saved weigh more than the launches and the merge that it takes (about 10 us, in
+  // which 32 MiB of keys come out of L2 again); otherwise each element walks them in the same pass as its own.
+  const bool pooled = s.B > 1 && rows < 128 && (int64_t)(s.B - 1) * s.Ls * s.Hkv * s.D * 4 > (32ll << 20);
   const int rows0 = pooled ? rows * s.B : rows;
   p.rows_per_tile = s.D == 64 && (rows0 <= kRowsKernelMax ? rows0 : rows) > 16 ? 32 : 16;
   auto fill = [&](int i, bool pool, bool sh, bool own, int part_rows) {
@@ -128,97 +129,99 @@ extern "C" int hb_context_workspace_bytes(int batch, int q_len, int kv_len, int 
   return HB_OK;
 }
 
-extern "C" int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, const void* kv,
-                               int64_t kv_batch_stride, int64_t kv_row_stride, const void* shared_kv,
-                               int64_t shared_row_stride, const int32_t* lens, const uint8_t* mask,
-                               int64_t mask_batch_stride, const uint8_t* shared_mask, const float* q_weight, float eps,
-                               float scale, void* out, int64_t out_batch_stride, int64_t out_row_stride, int batch,
-                               int q_len, int kv_len, int shared_len, int num_heads, int kv_heads, int head_dim,
-                               int dtype, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
-  if (!q || !out || (kv_len > 0 && !kv) || (shared_len > 0 && !shared_kv)) return HB_ERR_NULL;
-  const Shape s{batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim, mask || shared_mask ? 1 : 0};
-  if (!shape_ok(s) || (dtype != HB_BF16 && dtype != HB_FP16)) return HB_ERR_SHAPE;
-  if (!(scale > 0.f) || !std::isfinite(scale) || (q_weight && !(eps >= 0.f))) return HB_ERR_SHAPE;
-  const int64_t qw = (int64_t)num_heads * head_dim, kw = 2ll * kv_heads * head_dim;
-  if (q_row_stride < qw || out_row_stride < qw || (kv_len > 1 && kv_row_stride < kw) ||
-      (shared_len > 1 && shared_row_stride < kw) || q_batch_stride < 0 || kv_batch_stride < 0 ||
-      (mask && mask_batch_stride < 0))
+extern "C" int hb_context_attn(const HbContextArgs* args, cudaStream_t stream) {
+  if (!args) return HB_ERR_NULL;
+  const HbContextArgs& a = *args;
+  if (!a.q || !a.out || (a.kv_len > 0 && !a.kv) || (a.shared_len > 0 && !a.shared_kv)) return HB_ERR_NULL;
+  const Shape s{a.batch,     a.q_len,    a.kv_len,   a.shared_len,
+                a.num_heads, a.kv_heads, a.head_dim, a.mask || a.shared_mask ? 1 : 0};
+  if (!shape_ok(s) || (a.dtype != HB_BF16 && a.dtype != HB_FP16)) return HB_ERR_SHAPE;
+  if (!(a.scale > 0.f) || !std::isfinite(a.scale) || (a.q_weight && !(a.eps >= 0.f))) return HB_ERR_SHAPE;
+  const int64_t qw = (int64_t)a.num_heads * a.head_dim, kw = 2ll * a.kv_heads * a.head_dim;
+  if (a.q_row_stride < qw || a.out_row_stride < qw || (a.kv_len > 1 && a.kv_row_stride < kw) ||
+      (a.shared_len > 1 && a.shared_row_stride < kw) || a.q_batch_stride < 0 || a.kv_batch_stride < 0 ||
+      (a.mask && a.mask_batch_stride < 0))
     return HB_ERR_SHAPE;
   constexpr int64_t kMaxStride = (1ll << 39) - 1;  // a tensor map's: below 2^40 bytes
-  if (kv_batch_stride > kMaxStride || kv_row_stride > kMaxStride || shared_row_stride > kMaxStride) return HB_ERR_SHAPE;
-  // no two rows of the output share memory: batch elements one after the other, or interleaved row by row
-  if (batch > 1 && out_batch_stride < (q_len - 1) * out_row_stride + qw &&
-      (out_batch_stride < qw || out_row_stride < (batch - 1) * out_batch_stride + qw))
+  if (a.kv_batch_stride > kMaxStride || a.kv_row_stride > kMaxStride || a.shared_row_stride > kMaxStride)
     return HB_ERR_SHAPE;
-  const void* ptrs[] = {q, kv_len > 0 ? kv : nullptr, shared_len > 0 ? shared_kv : nullptr, out, workspace};
+  // no two rows of the output share memory: batch elements one after the other, or interleaved row by row
+  if (a.batch > 1 && a.out_batch_stride < (a.q_len - 1) * a.out_row_stride + qw &&
+      (a.out_batch_stride < qw || a.out_row_stride < (a.batch - 1) * a.out_batch_stride + qw))
+    return HB_ERR_SHAPE;
+  const void* ptrs[] = {a.q, a.kv_len > 0 ? a.kv : nullptr, a.shared_len > 0 ? a.shared_kv : nullptr, a.out,
+                        a.workspace};
   for (const void* pp : ptrs)
     if (pp && !aligned16(pp)) return HB_ERR_ALIGN;
-  if (reinterpret_cast<uintptr_t>(workspace) % 32) return HB_ERR_ALIGN;
-  if (q_batch_stride % 8 || q_row_stride % 8 || kv_batch_stride % 8 || kv_row_stride % 8 || shared_row_stride % 8 ||
-      out_batch_stride % 8 || out_row_stride % 8)
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 32) return HB_ERR_ALIGN;
+  if (a.q_batch_stride % 8 || a.q_row_stride % 8 || a.kv_batch_stride % 8 || a.kv_row_stride % 8 ||
+      a.shared_row_stride % 8 || a.out_batch_stride % 8 || a.out_row_stride % 8)
     return HB_ERR_ALIGN;
-  if ((reinterpret_cast<uintptr_t>(lens) & 3u) || (reinterpret_cast<uintptr_t>(q_weight) & 15u)) return HB_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(a.lens) & 3u) || (reinterpret_cast<uintptr_t>(a.q_weight) & 15u)) return HB_ERR_ALIGN;
   // What a tensor map describes: rows of at least their width; batch elements one after the other or interleaved
   // row by row, the larger stride a multiple of the smaller (or all of them the same rows: stride 0).
-  const bool inter = batch > 1 && kv_len > 1 && kv_batch_stride > 0 && kv_batch_stride < kv_row_stride;
-  if (batch > 1 && kv_len > 0 && kv_batch_stride > 0) {
-    if (kv_batch_stride < kw) return HB_ERR_SHAPE;
-    if (kv_len > 1 && (inter ? kv_row_stride % kv_batch_stride : kv_batch_stride % kv_row_stride)) return HB_ERR_ALIGN;
+  const bool inter = a.batch > 1 && a.kv_len > 1 && a.kv_batch_stride > 0 && a.kv_batch_stride < a.kv_row_stride;
+  if (a.batch > 1 && a.kv_len > 0 && a.kv_batch_stride > 0) {
+    if (a.kv_batch_stride < kw) return HB_ERR_SHAPE;
+    if (a.kv_len > 1 && (inter ? a.kv_row_stride % a.kv_batch_stride : a.kv_batch_stride % a.kv_row_stride))
+      return HB_ERR_ALIGN;
   }
   const Plan plan = make_plan(s);
-  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes)) return HB_ERR_WORKSPACE;
+  if (plan.bytes && (!a.workspace || a.workspace_bytes < 0 || static_cast<size_t>(a.workspace_bytes) < plan.bytes))
+    return HB_ERR_WORKSPACE;
   const int st = check_device();
   if (st != HB_OK) return st;
 
   CtxParams p{};
-  p.q = static_cast<const uint16_t*>(q);
-  p.q_bs = q_batch_stride;
-  p.q_rs = q_row_stride;
-  p.kv = static_cast<const uint16_t*>(kv);
-  p.kv_bs = kv_batch_stride;
-  p.kv_rs = kv_len > 1 ? kv_row_stride : std::max(kv_row_stride, kw);
-  if (kv_len == 1 && batch > 1 && kv_batch_stride > 0) p.kv_rs = kv_batch_stride;
+  p.q = static_cast<const uint16_t*>(a.q);
+  p.q_bs = a.q_batch_stride;
+  p.q_rs = a.q_row_stride;
+  p.kv = static_cast<const uint16_t*>(a.kv);
+  p.kv_bs = a.kv_batch_stride;
+  p.kv_rs = a.kv_len > 1 ? a.kv_row_stride : std::max(a.kv_row_stride, kw);
+  if (a.kv_len == 1 && a.batch > 1 && a.kv_batch_stride > 0) p.kv_rs = a.kv_batch_stride;
   p.kv_inter = inter;
-  p.skv = static_cast<const uint16_t*>(shared_kv);
-  p.skv_rs = shared_len > 1 ? shared_row_stride : std::max(shared_row_stride, kw);
-  p.lens = lens;
-  p.mask = mask;
-  p.mask_bs = mask_batch_stride;
-  p.smask = shared_mask;
-  p.q_w = q_weight;
-  p.eps = eps;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.out = static_cast<uint16_t*>(out);
-  p.o_bs = out_batch_stride;
-  p.o_rs = out_row_stride;
-  p.out_wide = reinterpret_cast<uintptr_t>(out) % 32 == 0 && out_row_stride % 16 == 0 && out_batch_stride % 16 == 0;
-  p.B = batch;
-  p.Lq = q_len;
-  p.H = num_heads;
-  p.Hkv = kv_heads;
-  p.G = num_heads / kv_heads;
-  p.Lkv = kv_len;
-  p.Ls = shared_len;
-  p.by_lq = fast_div(q_len);
+  p.skv = static_cast<const uint16_t*>(a.shared_kv);
+  p.skv_rs = a.shared_len > 1 ? a.shared_row_stride : std::max(a.shared_row_stride, kw);
+  p.lens = a.lens;
+  p.mask = a.mask;
+  p.mask_bs = a.mask_batch_stride;
+  p.smask = a.shared_mask;
+  p.q_w = a.q_weight;
+  p.eps = a.eps;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.out = static_cast<uint16_t*>(a.out);
+  p.o_bs = a.out_batch_stride;
+  p.o_rs = a.out_row_stride;
+  p.out_wide =
+      reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_row_stride % 16 == 0 && a.out_batch_stride % 16 == 0;
+  p.B = a.batch;
+  p.Lq = a.q_len;
+  p.H = a.num_heads;
+  p.Hkv = a.kv_heads;
+  p.G = a.num_heads / a.kv_heads;
+  p.Lkv = a.kv_len;
+  p.Ls = a.shared_len;
+  p.by_lq = fast_div(a.q_len);
   p.by_g = fast_div(p.G);
-  p.by_h = fast_div(num_heads);
-  p.by_hkv = fast_div(kv_heads);
+  p.by_h = fast_div(a.num_heads);
+  p.by_hkv = fast_div(a.kv_heads);
   p.slots = plan.slots;
   p.prows = plan.prows;
   p.tail_rows = plan.tail_rows;
-  p.o_part = static_cast<float*>(workspace);
-  if (plan.bytes) p.ml_part = reinterpret_cast<float2*>(p.o_part + (size_t)plan.slots * plan.prows * head_dim);
-  const bool fp16 = dtype == HB_FP16;
+  p.o_part = static_cast<float*>(a.workspace);
+  if (plan.bytes) p.ml_part = reinterpret_cast<float2*>(p.o_part + (size_t)plan.slots * plan.prows * a.head_dim);
+  const bool fp16 = a.dtype == HB_FP16;
   for (int kernel = 0; kernel < 2; ++kernel) {  // the parts of the few-rows kernel, then those of the tcgen05 one
     for (int i = 0; i < 2; ++i) {
       p.part[i] = plan.part[i];
       if (plan.tiles[i] != (kernel == 1)) p.part[i].count = 0;
     }
     if (p.part[0].count + p.part[1].count == 0) continue;
-    const int rc = kernel ? launch_ctx_tiles(p, head_dim, fp16, plan.mask_tiles, stream)
-                          : launch_ctx_rows(p, head_dim, fp16, plan.rows_per_tile, stream);
+    const int rc = kernel ? launch_ctx_tiles(p, a.head_dim, fp16, plan.mask_tiles, stream)
+                          : launch_ctx_rows(p, a.head_dim, fp16, plan.rows_per_tile, stream);
     if (rc != HB_OK) return rc;
   }
   p.part[1] = plan.part[1];
-  return plan.slots > 1 ? launch_ctx_combine(p, head_dim, fp16, stream) : HB_OK;
+  return plan.slots > 1 ? launch_ctx_combine(p, a.head_dim, fp16, stream) : HB_OK;
 }

@@ -386,9 +386,15 @@ __global__ void __launch_bounds__(256) ctx_combine_kernel(const CtxParams p) {
 
 template <int D, class T, int MT>
 int launch_rows(const CtxParams& p, cudaStream_t s) {
-  if (cudaFuncSetAttribute(ctx_rows_kernel<D, T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem) !=
-      cudaSuccess)
-    return HB_ERR_LAUNCH;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return HB_ERR_LAUNCH;
+  static bool configured[64] = {};
+  if (dev >= 64 || !configured[dev]) {
+    if (cudaFuncSetAttribute(ctx_rows_kernel<D, T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem) !=
+        cudaSuccess)
+      return HB_ERR_LAUNCH;
+    if (dev < 64) configured[dev] = true;
+  }
   ctx_rows_kernel<D, T, MT><<<p.part[0].count + p.part[1].count, 32 * kWarps, kRowsSmem, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }

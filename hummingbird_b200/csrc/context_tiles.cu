@@ -115,19 +115,23 @@ __device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
 // the limit is far above any wait of a working kernel; the loop stays a few instructions long because it is inlined
 // into every hot path (a longer one, with a clock, cost the kernel its instruction cache).
 constexpr uint32_t kWaitTries = 1u << 24;
+template <int kSleepNs>
 __device__ __forceinline__ bool slow_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
 #pragma unroll 1
-  for (uint32_t i = 0; i < kWaitTries && !*abort_flag; ++i)
+  for (uint32_t i = 0; i < kWaitTries && !*abort_flag; ++i) {
+    if (kSleepNs) __nanosleep(kSleepNs);
     if (mbar_try_wait(bar, parity)) return true;
+  }
   if (!*abort_flag) record_error(HB_ERR_TIMEOUT);
   *abort_flag = 1;
   return false;
 }
-__device__ __forceinline__ bool role_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return mbar_try_wait(bar, parity) || slow_wait(bar, parity, abort_flag);
+// The producer runs ahead: between tries it leaves the issue slots to the softmax.
+__device__ __forceinline__ bool producer_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return mbar_try_wait(bar, parity) || slow_wait<200>(bar, parity, abort_flag);
 }
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || slow_wait(bar, parity, abort_flag));
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || slow_wait<0>(bar, parity, abort_flag));
 }
 
 // A unit's key list: tiles [j0, j1) of the shared states' n0 tiles, then the batch element's own.
@@ -280,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
         const Keys ks = keys_of<kKeys>(p, part, u);
         const uint32_t* bits = bits0 + (n & 1) * mask_tiles * kWords;
         const int kcol = u.g * D, vcol = p.Hkv * D + u.g * D;
-        if (kMask && !(ok = role_wait(&m_full[n & 1], (n >> 1) & 1, abort_flag))) break;
+        if (kMask && !(ok = producer_wait(&m_full[n & 1], (n >> 1) & 1, abort_flag))) break;
         for (int j = ks.j0; j < ks.j1; ++j) {
           const Tile<kKeys> t = tile_of<kKeys, kMask>(p, ks, j, bits);
           if (t.hi <= 0) continue;
@@ -290,12 +294,12 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
           const bool inter = !t.shared && p.kv_inter;  // the map's second dimension is the batch
           const int bc = t.shared || p.kv_bs == 0 ? 0 : u.b;
           const int c1 = inter ? bc : t.k0, c2 = inter ? t.k0 : bc;
-          if (it >= kStages && !(ok = role_wait(&k_empty[st], ph, abort_flag))) break;
+          if (it >= kStages && !(ok = producer_wait(&k_empty[st], ph, abort_flag))) break;
           mbar_arrive_expect_tx(&k_full[st], L::kTile);
 #pragma unroll
           for (int h = 0; h < L::kHalves; ++h)
             tma_load_3d(smem + L::kOffK + st * L::kTile + h * L::kAtom, tm, kcol + 64 * h, c1, c2, &k_full[st]);
-          if (it >= kStages && !(ok = role_wait(&v_empty[st], ph, abort_flag))) {
+          if (it >= kStages && !(ok = producer_wait(&v_empty[st], ph, abort_flag))) {
             mbar_wait(&k_full[st], (it / kStages) & 1);  // K was issued already
             break;
           }
@@ -641,13 +645,19 @@ template <int D, bool kFp16, bool kMask>
 int launch_tiles(const CUtensorMap& own, const CUtensorMap& shared, const CtxParams& p, int mask_tiles,
                  cudaStream_t s) {
   auto kernel = ctx_tiles_kernel<D, kFp16, kMask>;
-  // setmaxnreg's split counts on exactly kLaunchRegs registers per thread at launch: an increase that the CTA's
-  // registers do not cover would never be granted
-  cudaFuncAttributes attr{};
-  if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess || attr.numRegs != Layout<D>::kLaunchRegs) return HB_ERR_LAUNCH;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::bytes(kCtxMaskTiles)) !=
-      cudaSuccess)
-    return HB_ERR_LAUNCH;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return HB_ERR_LAUNCH;
+  static bool configured[64] = {};
+  if (dev >= 64 || !configured[dev]) {
+    // setmaxnreg's split counts on exactly kLaunchRegs registers per thread at launch: an increase that the CTA's
+    // registers do not cover would never be granted
+    cudaFuncAttributes attr{};
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess || attr.numRegs != Layout<D>::kLaunchRegs ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::bytes(kCtxMaskTiles)) !=
+            cudaSuccess)
+      return HB_ERR_LAUNCH;
+    if (dev < 64) configured[dev] = true;
+  }
   const int grid = std::min(p.part[0].count + p.part[1].count, ctx_tile_ctas(D));
   kernel<<<grid, kThreads, Layout<D>::bytes(mask_tiles), s>>>(own, shared, p, mask_tiles);
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
@@ -680,9 +690,9 @@ int launch_ctx_tiles(const CtxParams& p, int D, bool fp16, int mask_tiles, cudaS
   if (use_own &&
       !(p.kv_inter ? encode_states(&own, p.kv, fp16, keys, width, batch, p.Lkv, p.kv_bs, p.kv_rs, true)
                    : encode_states(&own, p.kv, fp16, keys, width, p.Lkv, batch, p.kv_rs,
-                                   batch > 1 ? p.kv_bs : p.kv_rs * p.Lkv, false)))
+                                   batch > 1 ? p.kv_bs : p.kv_rs, false)))
     return HB_ERR_LAUNCH;
-  if (use_shared && !encode_states(&shared, p.skv, fp16, keys, width, p.Ls, 1, p.skv_rs, p.skv_rs * p.Ls, false))
+  if (use_shared && !encode_states(&shared, p.skv, fp16, keys, width, p.Ls, 1, p.skv_rs, p.skv_rs, false))
     return HB_ERR_LAUNCH;
   if (!use_own) own = shared;
   if (!use_shared) shared = own;

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from hummingbird_b200 import _lib
-from hummingbird_b200._tensors import check_cuda, stream_handle
+from hummingbird_b200._tensors import check_cuda, launch_on
 
 GROUPS = (32, 64, 128)
 _ACTS = {None: 0, "none": 0, "silu": 1}
@@ -34,12 +34,11 @@ def quantize_w4(weight: torch.Tensor, group: int = 128) -> tuple[torch.Tensor, t
     tiles, blocks = _blocks(n, k, group)
     check_cuda(weight)
     if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.stride(0) < k or weight.data_ptr() % 16:
-        weight = weight.contiguous() if not weight.is_contiguous() else weight.clone()
-    with torch.cuda.device(weight.device):
-        packed = torch.empty(tiles, blocks, 1024, dtype=torch.uint8, device=weight.device)
-        scales = torch.empty(tiles, blocks, 128 // group, 16, dtype=torch.bfloat16, device=weight.device)
-        _lib.call("hb_quant_w4", weight.data_ptr(), weight.stride(0), n, k, group, packed.data_ptr(),
-                  scales.data_ptr(), stream_handle(weight.device))
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    packed = torch.empty(tiles, blocks, 1024, dtype=torch.uint8, device=weight.device)
+    scales = torch.empty(tiles, blocks, 128 // group, 16, dtype=torch.bfloat16, device=weight.device)
+    launch_on(weight.get_device(), "hb_quant_w4", _lib.lib().hb_quant_w4, weight.data_ptr(), weight.stride(0), n, k,
+              group, packed.data_ptr(), scales.data_ptr())
     return packed, scales
 
 
@@ -67,11 +66,12 @@ def _check_weights(packed, scales, tiles, blocks, group):
                          f"{tuple(scales.shape)} {scales.dtype}")
 
 
-def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, out_features: int, group: int,
-              bias: torch.Tensor | None = None, *, act: str | None = None,
-              out: torch.Tensor | None = None) -> torch.Tensor:
-    """`act(x @ W^T + bias)` of bf16 or fp16 `x` `(M, K)` with the weights of `quantize_w4`: fp32 sums, one rounding
-    to x's type. `bias` `(N,)` of x's type; `act` "silu" or None ("none")."""
+_PLANS: dict = {}  # checked calls by the sizes, strides and types of their tensors
+_MAX_PLANS = 4096
+
+
+def _plan(x, packed, scales, out_features, group, bias, act, out):
+    """Check a call by its sizes and types: (copy x, copy bias, act code, type code)."""
     if x.dim() != 2 or x.dtype not in _DTYPES:
         raise ValueError(f"x must be bf16 or fp16 (M, K), got {tuple(x.shape)} {x.dtype}")
     if act not in _ACTS:
@@ -82,22 +82,46 @@ def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, out_f
         raise ValueError(f"bias must be {x.dtype} ({out_features},), got {tuple(bias.shape)} {bias.dtype}")
     if out is not None and (out.shape != (m, out_features) or out.dtype != x.dtype or out.stride(1) != 1):
         raise ValueError(f"out must be {x.dtype} ({m}, {out_features}) with unit stride in its last dim")
-    if any(t is not None and t.device != x.device for t in (packed, scales, bias, out)):
+    check_cuda(*(t for t in (x, packed, scales, bias, out) if t is not None))
+    return (x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.stride(0) < k, bias is not None and bias.stride(0) != 1,
+            _ACTS[act], _DTYPES[x.dtype])
+
+
+def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, out_features: int, group: int,
+              bias: torch.Tensor | None = None, *, act: str | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """`act(x @ W^T + bias)` of bf16 or fp16 `x` `(M, K)` with the weights of `quantize_w4`: fp32 sums, one rounding
+    to x's type. `bias` `(N,)` of x's type; `act` "silu" or None ("none")."""
+    key = (x.shape, x.stride(), x.dtype, packed.shape, packed.stride(), packed.dtype, scales.shape, scales.stride(),
+           scales.dtype, out_features, group, act, None if bias is None else (bias.shape, bias.stride(), bias.dtype),
+           None if out is None else (out.shape, out.stride(), out.dtype))
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = _plan(x, packed, scales, out_features, group, bias, act, out)
+        if len(_PLANS) >= _MAX_PLANS:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    copy_x, copy_bias, act_code, dtype_code = plan
+    device = x.get_device()
+    if device < 0 or packed.get_device() != device or scales.get_device() != device \
+            or (bias is not None and bias.get_device() != device) or (out is not None and out.get_device() != device):
+        check_cuda(*(t for t in (x, packed, scales, bias, out) if t is not None))
         raise ValueError("x, packed, scales, bias and out must be on one device")
-    check_cuda(x)
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+    if (x.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError("W4 linear layers have no backward pass: call them under torch.no_grad()")
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < k or x.data_ptr() % 16:
-        x = x.contiguous() if not x.is_contiguous() else x.clone()
-    if bias is not None and bias.stride(0) != 1:
+    x_at = x.data_ptr()
+    if copy_x or x_at & 15:
+        x = x.clone(memory_format=torch.contiguous_format)
+        x_at = x.data_ptr()
+    if copy_bias:
         bias = bias.contiguous()
+    m, k = x.shape
     if out is None:
-        out = torch.empty(m, out_features, dtype=x.dtype, device=x.device)
+        out = torch.empty((m, out_features), dtype=x.dtype, device=x.device)
     if m:
-        with torch.cuda.device(x.device):
-            _lib.call("hb_w4_linear", x.data_ptr(), x.stride(0), packed.data_ptr(), scales.data_ptr(),
-                      None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0), m, out_features, k,
-                      group, _ACTS[act], _DTYPES[x.dtype], stream_handle(x.device))
+        launch_on(device, "hb_w4_linear", _lib.lib().hb_w4_linear, x_at, x.stride(0), packed.data_ptr(),
+                  scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0), m,
+                  out_features, k, group, act_code, dtype_code)
     return out
 
 

@@ -110,6 +110,27 @@ int hb_cross_diff_attn(const void* q, int64_t q_row_stride, const void* kv, int6
 int hb_context_workspace_bytes(int batch, int q_len, int kv_len, int shared_len, int num_heads, int kv_heads,
                                int head_dim, int masked, size_t* bytes);
 
+/* A call of hb_context_attn: one struct, because foreign calls from Python cost by the argument. */
+typedef struct HbContextArgs {
+  const void* q;
+  const void* kv;
+  const void* shared_kv;
+  const int32_t* lens;
+  const uint8_t* mask;
+  const uint8_t* shared_mask;
+  const float* q_weight;
+  void* out;
+  void* workspace;
+  int64_t q_batch_stride, q_row_stride;
+  int64_t kv_batch_stride, kv_row_stride;
+  int64_t shared_row_stride;
+  int64_t mask_batch_stride;
+  int64_t out_batch_stride, out_row_stride;
+  int64_t workspace_bytes;
+  int batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim, dtype;
+  float eps, scale;
+} HbContextArgs;
+
 /* The attention of `sa3jax.dit._cross_attention` (dit.py:203-215) in its non-differential form (`_attend_out`'s
  * plain `SDPA(q, k, v)`, dit.py:131-147), up to (not including) `to_out`, for contexts of any length, padded
  * batches, fewer kv heads than query heads, and states that the whole batch shares:
@@ -127,17 +148,11 @@ int hb_context_workspace_bytes(int batch, int q_len, int kv_len, int shared_len,
  *   dtype     HB_BF16 or HB_FP16, for q, kv, shared_kv and out alike.
  * A row without a valid key is written as zeros; what lies at keys that are not valid (infinities, NaN) does not
  * reach the result. Scores, softmax statistics and sums are fp32; the weights p are rounded to the 16-bit type for
- * the product with v (relative error at most 2^-8 or 2^-11 each), the sum of p is not. head_dim 64 or 128; rows of q, kv,
- * shared_kv, out and their strides 16-byte aligned, workspace 32-byte; kv's batch stride 0, or one of its two strides a multiple of the
- * other; kv_len and shared_len at most 2^24; scale > 0. The result does not depend on timing: the same call
- * gives the same bits. Calls that may overlap on the GPU need workspaces of their own. */
-int hb_context_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, const void* kv,
-                    int64_t kv_batch_stride, int64_t kv_row_stride, const void* shared_kv, int64_t shared_row_stride,
-                    const int32_t* lens, const uint8_t* mask, int64_t mask_batch_stride, const uint8_t* shared_mask,
-                    const float* q_weight, float eps, float scale, void* out, int64_t out_batch_stride,
-                    int64_t out_row_stride, int batch, int q_len, int kv_len, int shared_len, int num_heads,
-                    int kv_heads, int head_dim, int dtype, void* workspace, size_t workspace_bytes,
-                    cudaStream_t stream);
+ * the product with v (relative error at most 2^-8 or 2^-11 each), the sum of p is not. head_dim 64 or 128; rows of q,
+ * kv, shared_kv, out and their strides 16-byte aligned, workspace 32-byte; kv's batch stride 0, or one of its two
+ * strides a multiple of the other; kv_len and shared_len at most 2^24; scale > 0. The result does not depend on
+ * timing: the same call gives the same bits. Calls that may overlap on the GPU need workspaces of their own. */
+int hb_context_attn(const HbContextArgs* args, cudaStream_t stream);
 
 /* ---- band (sliding-window) differential attention (SAME-L decoder) --------------------------------- */
 /* Bytes of workspace hb_band_diff_attn needs for `rows` buffer rows, `pair_count` head pairs, `window` and

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from hummingbird_b200 import _lib
+from hummingbird_b200.context_attention import _ARGS
 
 P = 0x7F0000001000
 
@@ -24,12 +25,13 @@ def _need(lib, *sizes, masked=0):
 
 
 def _args(**kw):
-    a = dict(q=P, q_bs=300 * 1024, q_rs=1024, kv=P, kv_bs=257 * 2048, kv_rs=2048, skv=None, skv_rs=0, lens=None,
-             mask=None, mask_bs=0, smask=None, q_w=None, eps=1e-6, scale=0.125, out=P, o_bs=300 * 1024, o_rs=1024,
-             batch=2, q_len=300, kv_len=257, shared_len=0, heads=16, kv_heads=16, head_dim=64, dtype=_lib.HB_BF16,
-             ws=P, ws_bytes=1 << 40, stream=None)
+    a = dict(q=P, kv=P, skv=0, lens=0, mask=0, smask=0, q_w=0, out=P, ws=P, q_bs=300 * 1024, q_rs=1024,
+             kv_bs=257 * 2048, kv_rs=2048, skv_rs=0, mask_bs=0, o_bs=300 * 1024, o_rs=1024, ws_bytes=1 << 40, batch=2,
+             q_len=300, kv_len=257, shared_len=0, heads=16, kv_heads=16, head_dim=64, dtype=_lib.HB_BF16, eps=1e-6,
+             scale=0.125)
+    assert set(kw) <= set(a)
     a.update(kw)
-    return list(a.values())
+    return _ARGS.pack(*(0 if v is None else v for v in a.values())), None
 
 
 @pytest.mark.parametrize("override,status", [
@@ -62,6 +64,7 @@ def _args(**kw):
     (dict(kv_bs=2056, kv_rs=4096), _lib.HB_ERR_ALIGN),
     (dict(kv_rs=1 << 40), _lib.HB_ERR_SHAPE),
     (dict(q=P + 8), _lib.HB_ERR_ALIGN),
+    (dict(ws=P + 16), _lib.HB_ERR_ALIGN),
     (dict(kv=P + 2), _lib.HB_ERR_ALIGN),
     (dict(out=P + 4), _lib.HB_ERR_ALIGN),
     (dict(q_rs=1028), _lib.HB_ERR_ALIGN),
@@ -71,6 +74,11 @@ def _args(**kw):
 ])
 def test_rejects(lib, override, status):
     assert lib.hb_context_attn(*_args(**override)) == status
+
+
+def test_struct_has_the_header_s_size_and_null_is_refused(lib):
+    assert _ARGS.size == 9 * 8 + 9 * 8 + 8 * 4 + 2 * 4
+    assert lib.hb_context_attn(None, None) == _lib.HB_ERR_NULL
 
 
 def test_workspace_is_asked_for_and_checked(lib):
