@@ -27,14 +27,13 @@ except ImportError:
         return torch.cuda.current_stream(device).cuda_stream
 
 
-def launch_on(device: int, name: str, fn, *args) -> None:
-    """Call entry point `fn` with its arguments and the current stream of CUDA device `device`, with that device
-    current."""
+def launch(device: int, name: str, fn, args) -> None:
+    """Call entry point `fn(args, stream)` on the current stream of CUDA device `device`, with that device current."""
     if torch.cuda.current_device() == device:
-        code = fn(*args, raw_stream(device))
+        code = fn(args, raw_stream(device))
     else:
         with torch.cuda.device(device):
-            code = fn(*args, raw_stream(device))
+            code = fn(args, raw_stream(device))
     if code:
         _lib.check(name, code)
 

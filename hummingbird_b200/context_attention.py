@@ -18,7 +18,7 @@ import struct
 import torch
 
 from hummingbird_b200 import _lib
-from hummingbird_b200._tensors import check_cuda, launch_on
+from hummingbird_b200._tensors import check_cuda, launch
 
 _DTYPES = {torch.bfloat16: _lib.HB_BF16, torch.float16: _lib.HB_FP16}
 _ARGS = struct.Struct("=9Q9q8i2f")  # HbContextArgs: pointers, strides, sizes, eps and scale
@@ -116,7 +116,7 @@ def _attend(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_
     weight_at = 0 if q_weight is None else q_weight.data_ptr()
     if copies or (q_at | kv_at | shared_at | weight_at) & 15:
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = q.new_empty(q.shape)
         c = copies or (False,) * 7
         return _attend(_own_copy(q, c[0] or q_at & 15), shared_kv if shared_kv is None else
                        _own_copy(shared_kv, c[2] or shared_at & 15), _own_copy(kv, c[1] or kv_at & 15), num_heads,
@@ -126,18 +126,18 @@ def _attend(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_
                        q_weight if q_weight is None else _own_copy(q_weight, c[6] or weight_at & 15, torch.float32),
                        eps, scale, out)
     if out is None:
-        out = torch.empty_like(q) if like_q else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if like_q else q.new_empty(q.shape)
     if not sizes[0] or not sizes[1]:
         return out
     # Partial results in a block of the caching allocator: it belongs to this call's stream, or to the graph that is
     # being captured, so calls on other streams and other graphs have theirs.
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     out_strides = out.stride()
     args = _ARGS.pack(q_at, kv_at, shared_at, 0 if lens is None else lens.data_ptr(),
                       0 if mask is None else mask.data_ptr(), 0 if shared_mask is None else shared_mask.data_ptr(),
                       weight_at, out.data_ptr(), 0 if ws is None else ws.data_ptr(), *strides, out_strides[0],
                       out_strides[1], need, *sizes, eps, head_dim ** -0.5 if scale is None else scale)
-    launch_on(device, "hb_context_attn", _lib.lib().hb_context_attn, args)
+    launch(device, "hb_context_attn", _lib.lib().hb_context_attn, args)
     return out
 
 

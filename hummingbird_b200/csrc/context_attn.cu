@@ -212,14 +212,16 @@ extern "C" int hb_context_attn(const HbContextArgs* args, cudaStream_t stream) {
   p.o_part = static_cast<float*>(a.workspace);
   if (plan.bytes) p.ml_part = reinterpret_cast<float2*>(p.o_part + (size_t)plan.slots * plan.prows * a.head_dim);
   const bool fp16 = a.dtype == HB_FP16;
+  bool launched = false;
   for (int kernel = 0; kernel < 2; ++kernel) {  // the parts of the few-rows kernel, then those of the tcgen05 one
     for (int i = 0; i < 2; ++i) {
       p.part[i] = plan.part[i];
       if (plan.tiles[i] != (kernel == 1)) p.part[i].count = 0;
     }
     if (p.part[0].count + p.part[1].count == 0) continue;
-    const int rc = kernel ? launch_ctx_tiles(p, a.head_dim, fp16, plan.mask_tiles, stream)
+    const int rc = kernel ? launch_ctx_tiles(p, a.head_dim, fp16, plan.mask_tiles, launched, stream)
                           : launch_ctx_rows(p, a.head_dim, fp16, plan.rows_per_tile, stream);
+    launched = true;
     if (rc != HB_OK) return rc;
   }
   p.part[1] = plan.part[1];

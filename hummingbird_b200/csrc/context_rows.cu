@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
   uint32_t* bits_s = reinterpret_cast<uint32_t*>(smem + kWarps * kWarpBytes);
   float2* ml_s = reinterpret_cast<float2*>(smem + kWarps * kWarpBytes + kWarps * kStages * 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the tcgen05 kernel beside it, or the merge
 
   // ---- which item
   const bool second = static_cast<int>(blockIdx.x) >= p.part[0].count;
@@ -340,43 +341,71 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
   }
 }
 
-// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s in slot order; four elements of a row per thread.
-template <int D, class T>
+// out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s; four elements of a row per thread, kTeams teams of D / 4 threads
+// to a row, which take every kTeams-th slot and join in order: a long list of slots would otherwise be one thread's.
+template <int D, class T, int kTeams>
 __global__ void __launch_bounds__(256) ctx_combine_kernel(const CtxParams p) {
   constexpr int TPR = D / 4;
-  const int row = static_cast<int>(((int64_t)blockIdx.x * 256 + threadIdx.x) / TPR);
-  const int ch = threadIdx.x % TPR;
-  if (row >= p.prows) return;
-  CtxRow x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial results of every kernel of this call
+  __shared__ float4 acc_s[256];
+  __shared__ float2 ml_s[256];
+  const int idx = static_cast<int>(((int64_t)blockIdx.x * 256 + threadIdx.x) / TPR);
+  const int row = idx / kTeams, team = idx % kTeams, ch = threadIdx.x % TPR;
+  bool live = row < p.prows;
+  CtxRow x{};
   if (p.tail_rows) {
     const CtxPart& part = p.part[1];
     const int i = row / p.tail_rows;
-    const CtxUnit u = ctx_unit(p, part, i * part.splits);
+    const CtxUnit u = ctx_unit(p, part, live ? i * part.splits : 0);
     const int r = u.rt * p.tail_rows + (row - i * p.tail_rows);
-    if (r >= u.rows) return;
-    x = ctx_row(p, r, u.g, u.b, part.pooled);
-  } else {
+    live = live && r < u.rows;
+    if (live) x = ctx_row(p, r, u.g, u.b, part.pooled);
+  } else if (live) {
     const int t = p.by_h.div(row);
     x.hq = row - t * p.H;
     x.bq = p.by_lq.div(t);
     x.i = t - x.bq * p.Lq;
   }
-  float mx = -INFINITY;
-  for (int s = 0; s < p.slots; ++s) mx = fmaxf(mx, p.ml_part[(int64_t)s * p.prows + row].x);
-  float sum = 0.f;
+  float mx = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+    for (int s = team; s < p.slots; s += kTeams) mx = fmaxf(mx, p.ml_part[(int64_t)s * p.prows + row].x);
 #pragma unroll 4
-  for (int s = 0; s < p.slots; ++s) {
-    const float2 ml = p.ml_part[(int64_t)s * p.prows + row];
-    if (ml.x == -INFINITY) continue;  // a part without keys left its sums unwritten
-    const float f = ex2_approx(ml.x - mx);
-    const float4 v = *reinterpret_cast<const float4*>(p.o_part + ((int64_t)s * p.prows + row) * D + ch * 4);
-    sum = fmaf(f, ml.y, sum);
-    acc.x = fmaf(f, v.x, acc.x);
-    acc.y = fmaf(f, v.y, acc.y);
-    acc.z = fmaf(f, v.z, acc.z);
-    acc.w = fmaf(f, v.w, acc.w);
+    for (int s = team; s < p.slots; s += kTeams) {
+      const float2 ml = p.ml_part[(int64_t)s * p.prows + row];
+      if (ml.x == -INFINITY) continue;  // a part without keys left its sums unwritten
+      const float f = ex2_approx(ml.x - mx);
+      const float4 v = *reinterpret_cast<const float4*>(p.o_part + ((int64_t)s * p.prows + row) * D + ch * 4);
+      sum = fmaf(f, ml.y, sum);
+      acc.x = fmaf(f, v.x, acc.x);
+      acc.y = fmaf(f, v.y, acc.y);
+      acc.z = fmaf(f, v.z, acc.z);
+      acc.w = fmaf(f, v.w, acc.w);
+    }
   }
+  if constexpr (kTeams > 1) {
+    acc_s[threadIdx.x] = acc;
+    ml_s[threadIdx.x] = make_float2(mx, sum);
+    __syncthreads();
+    if (!live || team) return;
+#pragma unroll
+    for (int k = 1; k < kTeams; ++k) mx = fmaxf(mx, ml_s[threadIdx.x + k * TPR].x);
+    sum = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kTeams; ++k) {
+      const float2 ml = ml_s[threadIdx.x + k * TPR];
+      if (ml.x == -INFINITY) continue;
+      const float f = ex2_approx(ml.x - mx);
+      const float4 v = acc_s[threadIdx.x + k * TPR];
+      sum = fmaf(f, ml.y, sum);
+      acc.x = fmaf(f, v.x, acc.x);
+      acc.y = fmaf(f, v.y, acc.y);
+      acc.z = fmaf(f, v.z, acc.z);
+      acc.w = fmaf(f, v.w, acc.w);
+    }
+  }
+  if (!live) return;
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
   uint2 w;
   w.x = T::pack(acc.x * inv, acc.y * inv);
@@ -399,11 +428,18 @@ int launch_rows(const CtxParams& p, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 
+template <int D, class T, int kTeams>
+int launch_teams(const CtxParams& p, cudaStream_t s) {
+  const int64_t threads = (int64_t)p.prows * (D / 4) * kTeams;
+  return ctx_launch_after(ctx_combine_kernel<D, T, kTeams>, static_cast<unsigned>((threads + 255) / 256), 256, 0, s, p);
+}
+// As many teams as it takes to have about a thousand threads on every SM, and no more than have slots to read.
 template <int D, class T>
 int launch_combine(const CtxParams& p, cudaStream_t s) {
-  const int64_t threads = (int64_t)p.prows * (D / 4);
-  ctx_combine_kernel<D, T><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
+  const int64_t threads = (int64_t)p.prows * (D / 4), want = kCtxSms * 1024;
+  if (p.slots <= 4 || threads >= want) return launch_teams<D, T, 1>(p, s);
+  if (p.slots <= 16 || 4 * threads >= want) return launch_teams<D, T, 4>(p, s);
+  return launch_teams<D, T, 1024 / D>(p, s);
 }
 
 }  // namespace

@@ -215,6 +215,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
   uint32_t* bits0 = reinterpret_cast<uint32_t*>(smem + L::kOffBits);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge
   const int count0 = p.part[0].count, total = count0 + p.part[1].count;
 
   if (warp == 4 && lane == 0) {
@@ -611,6 +612,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
     tc_fence_after();
     tmem_dealloc(tmem, L::kTmemCols);
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the few-rows kernel, where this one was launched beside it
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -643,7 +645,7 @@ bool encode_states(CUtensorMap* map, const void* base, bool fp16, unsigned keys,
 
 template <int D, bool kFp16, bool kMask>
 int launch_tiles(const CUtensorMap& own, const CUtensorMap& shared, const CtxParams& p, int mask_tiles,
-                 cudaStream_t s) {
+                 bool beside, cudaStream_t s) {
   auto kernel = ctx_tiles_kernel<D, kFp16, kMask>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return HB_ERR_LAUNCH;
@@ -659,15 +661,16 @@ int launch_tiles(const CUtensorMap& own, const CUtensorMap& shared, const CtxPar
     if (dev < 64) configured[dev] = true;
   }
   const int grid = std::min(p.part[0].count + p.part[1].count, ctx_tile_ctas(D));
+  if (beside) return ctx_launch_after(kernel, grid, kThreads, Layout<D>::bytes(mask_tiles), s, own, shared, p, mask_tiles);
   kernel<<<grid, kThreads, Layout<D>::bytes(mask_tiles), s>>>(own, shared, p, mask_tiles);
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 
 template <int D, bool kFp16>
 int launch_tiles(const CUtensorMap& own, const CUtensorMap& shared, const CtxParams& p, bool mask, int mask_tiles,
-                 cudaStream_t s) {
-  return mask ? launch_tiles<D, kFp16, true>(own, shared, p, mask_tiles, s)
-              : launch_tiles<D, kFp16, false>(own, shared, p, 0, s);
+                 bool beside, cudaStream_t s) {
+  return mask ? launch_tiles<D, kFp16, true>(own, shared, p, mask_tiles, beside, s)
+              : launch_tiles<D, kFp16, false>(own, shared, p, 0, beside, s);
 }
 
 }  // namespace
@@ -680,7 +683,7 @@ int ctx_tiles_take_status(unsigned int* status) {
   return HB_OK;
 }
 
-int launch_ctx_tiles(const CtxParams& p, int D, bool fp16, int mask_tiles, cudaStream_t s) {
+int launch_ctx_tiles(const CtxParams& p, int D, bool fp16, int mask_tiles, bool beside, cudaStream_t s) {
   const int64_t width = 2ll * p.Hkv * D;
   const unsigned keys = ctx_tile_keys(D);
   CUtensorMap own{}, shared{};
@@ -698,10 +701,10 @@ int launch_ctx_tiles(const CtxParams& p, int D, bool fp16, int mask_tiles, cudaS
   if (!use_shared) shared = own;
   const bool mask = p.mask || p.smask;
   if (D == 128)
-    return fp16 ? launch_tiles<128, true>(own, shared, p, mask, mask_tiles, s)
-                : launch_tiles<128, false>(own, shared, p, mask, mask_tiles, s);
-  return fp16 ? launch_tiles<64, true>(own, shared, p, mask, mask_tiles, s)
-              : launch_tiles<64, false>(own, shared, p, mask, mask_tiles, s);
+    return fp16 ? launch_tiles<128, true>(own, shared, p, mask, mask_tiles, beside, s)
+                : launch_tiles<128, false>(own, shared, p, mask, mask_tiles, beside, s);
+  return fp16 ? launch_tiles<64, true>(own, shared, p, mask, mask_tiles, beside, s)
+              : launch_tiles<64, false>(own, shared, p, mask, mask_tiles, beside, s);
 }
 
 }  // namespace hb

@@ -12,9 +12,9 @@
 // or-ed into the mantissa of 128 (bf16) or 1024 (fp16) and 136 or 1032 subtracted: q exactly, without a conversion.
 // Each group's sum is accumulated by the MMAs in fp32 and multiplied by its scale once, in fp32.
 //
-// One CTA takes 16 outputs; its eight warps take every eighth block of 128 inputs and merge through shared memory
-// in warp order, so the result does not depend on timing. x is read through L1 (it is the same few rows for
-// every CTA).
+// One CTA takes 16 outputs; its eight warps take every eighth block of 128 inputs, each through a ring of asynchronous
+// copies of its own, and merge through shared memory in warp order, so the result does not depend on timing. x is
+// read through L1 (it is the same few rows for every CTA).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,6 +28,7 @@ namespace hb {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kStages = 4;  // blocks of a warp on their way
 
 struct W4Params {
   const uint16_t* x;
@@ -77,11 +78,19 @@ struct Half<true> {
   static __device__ __forceinline__ uint16_t round(float v) { return __half_as_ushort(__float2half_rn(v)); }
 };
 
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 template <bool kFp16, int NT, int kGroup>
 __global__ void __launch_bounds__(32 * kWarps) w4_linear_kernel(const W4Params p) {
   using T = Half<kFp16>;
-  constexpr int kSteps = kGroup / 32;  // word steps per group
-  __shared__ float part[kWarps][16][8 * NT + 1];
+  constexpr int kSteps = kGroup / 32;        // word steps per group
+  constexpr int kGroups = 128 / kGroup;      // groups per block
+  constexpr int kStageBytes = 1024 + 32 * kGroups;
+  constexpr int kRing = kStages * kStageBytes;
+  constexpr int kPart = 16 * (8 * NT + 1) * 4;
+  __shared__ __align__(16) uint8_t smem[kWarps * (kRing > kPart ? kRing : kPart)];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
   const int tile = blockIdx.x, m0 = blockIdx.y * 8 * NT;
 
@@ -91,8 +100,25 @@ __global__ void __launch_bounds__(32 * kWarps) w4_linear_kernel(const W4Params p
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
 
-  const uint4* wp = p.packed + (int64_t)tile * p.kblocks * 64 + lane;
-  const uint16_t* sp = p.scales + (int64_t)tile * p.kblocks * (2048 / kGroup) + gid;
+  // Each warp's blocks through a ring of its own: a lane copies what it reads of the weights itself, the scales are
+  // read by all.
+  const uint8_t* wp = reinterpret_cast<const uint8_t*>(p.packed) + (int64_t)tile * p.kblocks * 1024 + lane * 16;
+  const uint8_t* sp = reinterpret_cast<const uint8_t*>(p.scales) + (int64_t)tile * p.kblocks * (32 * kGroups) +
+                      (lane < 2 * kGroups ? lane * 16 : 0);
+  const uint8_t* ring = smem + warp * kRing;
+  const uint32_t ring_at = smem_u32(ring);
+  auto load = [&](int kb, int st) {  // one commit group, also where nothing is copied
+    if (kb < p.kblocks) {
+      const uint32_t dst = ring_at + st * kStageBytes + lane * 16;
+      cp16(dst, wp + (int64_t)kb * 1024);
+      cp16(dst + 512, wp + (int64_t)kb * 1024 + 512);
+      if (lane < 2 * kGroups) cp16(dst + 1024, sp + (int64_t)kb * (32 * kGroups));
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) load(warp + s * kWarps, s);
+
   const uint16_t* xp[NT];
   bool live[NT];
 #pragma unroll
@@ -101,27 +127,10 @@ __global__ void __launch_bounds__(32 * kWarps) w4_linear_kernel(const W4Params p
     live[t] = m < p.M;
     xp[t] = p.x + (live[t] ? m : 0) * p.ldx + tid * 8;
   }
-
-  uint4 wa, wb;
-  int kb = warp;
-  if (kb < p.kblocks) {
-    wa = ld_nc_v4(wp + (int64_t)kb * 64);
-    wb = ld_nc_v4(wp + (int64_t)kb * 64 + 32);
-  }
-  while (kb < p.kblocks) {
-    const uint32_t lo[4] = {wa.x, wa.y, wa.z, wa.w}, hi[4] = {wb.x, wb.y, wb.z, wb.w};
-    const int k0 = kb * 128, next = kb + kWarps;
-    if (next < p.kblocks) {
-      wa = ld_nc_v4(wp + (int64_t)next * 64);
-      wb = ld_nc_v4(wp + (int64_t)next * 64 + 32);
-    }
-    float sc[128 / kGroup][2];
-#pragma unroll
-    for (int g = 0; g < 128 / kGroup; ++g) {
-      const uint16_t* s = sp + ((int64_t)kb * (128 / kGroup) + g) * 16;
-      sc[g][0] = __uint_as_float((uint32_t)__ldg(s) << 16);
-      sc[g][1] = __uint_as_float((uint32_t)__ldg(s + 8) << 16);
-    }
+  int st = 0;
+  for (int kb = warp; kb < p.kblocks; kb += kWarps) {
+    load(kb + (kStages - 1) * kWarps, st == 0 ? kStages - 1 : st - 1);
+    const int k0 = kb * 128;
     uint4 xv[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -129,8 +138,15 @@ __global__ void __launch_bounds__(32 * kWarps) w4_linear_kernel(const W4Params p
       for (int w = 0; w < 4; ++w)
         xv[t][w] = live[t] && k0 + 32 * w < p.K ? __ldg(reinterpret_cast<const uint4*>(xp[t] + k0 + 32 * w))
                                                 : make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    __syncwarp();
+    const uint8_t* stage = ring + st * kStageBytes;
+    const uint4 wa = *reinterpret_cast<const uint4*>(stage + lane * 16);
+    const uint4 wb = *reinterpret_cast<const uint4*>(stage + 512 + lane * 16);
+    const uint32_t lo[4] = {wa.x, wa.y, wa.z, wa.w}, hi[4] = {wb.x, wb.y, wb.z, wb.w};
+    const uint16_t* sc = reinterpret_cast<const uint16_t*>(stage + 1024) + gid;
 #pragma unroll
-    for (int g = 0; g < 128 / kGroup; ++g) {
+    for (int g = 0; g < kGroups; ++g) {
       float c[NT][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -148,24 +164,30 @@ __global__ void __launch_bounds__(32 * kWarps) w4_linear_kernel(const W4Params p
           T::mma(c[t], a1, xv[t][w].z, xv[t][w].w);
         }
       }
+      const float s0 = __uint_as_float((uint32_t)sc[g * 16] << 16), s1 = __uint_as_float((uint32_t)sc[g * 16 + 8] << 16);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(sc[g][e >> 1], c[t][e], acc[t][e]);
+        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(e < 2 ? s0 : s1, c[t][e], acc[t][e]);
     }
-    kb = next;
+    __syncwarp();  // every lane has read the stage's scales before it is filled again
+    if (++st == kStages) st = 0;
   }
+  __syncthreads();  // (the copies still in flight are empty groups) the rings become the partial sums
+  float* part = reinterpret_cast<float*>(smem);
+  constexpr int kRow = 8 * NT + 1, kWarp = 16 * kRow;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[warp][gid + 8 * (e >> 1)][t * 8 + tid * 2 + (e & 1)] = acc[t][e];
+    for (int e = 0; e < 4; ++e)
+      part[warp * kWarp + (gid + 8 * (e >> 1)) * kRow + t * 8 + tid * 2 + (e & 1)] = acc[t][e];
   __syncthreads();
   const int warps = min(kWarps, p.kblocks);
   for (int i = threadIdx.x; i < 128 * NT; i += 32 * kWarps) {
     const int r = i & 15, c = i >> 4, n = tile * 16 + r, m = m0 + c;
     if (n >= p.N || m >= p.M) continue;
-    float v = part[0][r][c];
-    for (int w = 1; w < warps; ++w) v += part[w][r][c];
+    float v = part[r * kRow + c];
+    for (int w = 1; w < warps; ++w) v += part[w * kWarp + r * kRow + c];
     if (p.bias) v += T::load(p.bias + n);
     if (p.silu) v = v / (1.f + expf(-v));
     p.y[m * p.ldy + n] = T::round(v);
@@ -257,26 +279,35 @@ extern "C" int hb_quant_w4(const void* w, int64_t ldw, int N, int K, int group, 
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 
-extern "C" int hb_w4_linear(const void* x, int64_t ldx, const void* packed, const void* scales, const void* bias,
-                            void* y, int64_t ldy, int M, int N, int K, int group, int silu, int dtype,
-                            cudaStream_t stream) {
-  if (!x || !packed || !scales || !y) return HB_ERR_NULL;
-  if (!w4_shape_ok(N, K, group) || M < 1 || M > 32 * 65535 || ldx < K || ldy < N ||
-      (dtype != HB_BF16 && dtype != HB_FP16) || (silu != 0 && silu != 1))
+extern "C" int hb_w4_linear(const HbW4Args* args, cudaStream_t stream) {
+  if (!args) return HB_ERR_NULL;
+  const HbW4Args& a = *args;
+  if (!a.x || !a.packed || !a.scales || !a.y) return HB_ERR_NULL;
+  if (!w4_shape_ok(a.N, a.K, a.group) || a.M < 1 || a.M > 32 * 65535 || a.ldx < a.K || a.ldy < a.N ||
+      (a.dtype != HB_BF16 && a.dtype != HB_FP16) || (a.silu != 0 && a.silu != 1))
     return HB_ERR_SHAPE;
-  if (!aligned16(x) || !aligned16(packed) || !aligned16(scales) || ldx % 8 || (reinterpret_cast<uintptr_t>(y) & 1u) ||
-      (reinterpret_cast<uintptr_t>(bias) & 1u))
+  if (!aligned16(a.x) || !aligned16(a.packed) || !aligned16(a.scales) || a.ldx % 8 ||
+      (reinterpret_cast<uintptr_t>(a.y) & 1u) || (reinterpret_cast<uintptr_t>(a.bias) & 1u))
     return HB_ERR_ALIGN;
   const int st = check_device();
   if (st != HB_OK) return st;
-  const W4Params p{static_cast<const uint16_t*>(x), ldx, static_cast<const uint4*>(packed),
-                   static_cast<const uint16_t*>(scales), static_cast<const uint16_t*>(bias),
-                   static_cast<uint16_t*>(y), ldy, M, N, K, (K + 127) / 128, silu};
-  const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4;
-  const dim3 grid((N + 15) / 16, (M + 8 * nt - 1) / (8 * nt));
-  if (dtype == HB_FP16)
-    launch_linear<true>(p, nt, group, grid, stream);
+  const W4Params p{static_cast<const uint16_t*>(a.x),
+                   a.ldx,
+                   static_cast<const uint4*>(a.packed),
+                   static_cast<const uint16_t*>(a.scales),
+                   static_cast<const uint16_t*>(a.bias),
+                   static_cast<uint16_t*>(a.y),
+                   a.ldy,
+                   a.M,
+                   a.N,
+                   a.K,
+                   (a.K + 127) / 128,
+                   a.silu};
+  const int nt = a.M <= 8 ? 1 : a.M <= 16 ? 2 : 4;
+  const dim3 grid((a.N + 15) / 16, (a.M + 8 * nt - 1) / (8 * nt));
+  if (a.dtype == HB_FP16)
+    launch_linear<true>(p, nt, a.group, grid, stream);
   else
-    launch_linear<false>(p, nt, group, grid, stream);
+    launch_linear<false>(p, nt, a.group, grid, stream);
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }

@@ -7,11 +7,14 @@ and laid out once (`quantize_w4`).
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from hummingbird_b200 import _lib
-from hummingbird_b200._tensors import check_cuda, launch_on
+from hummingbird_b200._tensors import check_cuda, launch, stream_handle
 
+_ARGS = struct.Struct("=5Q2q6i")  # HbW4Args
 GROUPS = (32, 64, 128)
 _ACTS = {None: 0, "none": 0, "silu": 1}
 _DTYPES = {torch.bfloat16: _lib.HB_BF16, torch.float16: _lib.HB_FP16}
@@ -37,8 +40,9 @@ def quantize_w4(weight: torch.Tensor, group: int = 128) -> tuple[torch.Tensor, t
         weight = weight.clone(memory_format=torch.contiguous_format)
     packed = torch.empty(tiles, blocks, 1024, dtype=torch.uint8, device=weight.device)
     scales = torch.empty(tiles, blocks, 128 // group, 16, dtype=torch.bfloat16, device=weight.device)
-    launch_on(weight.get_device(), "hb_quant_w4", _lib.lib().hb_quant_w4, weight.data_ptr(), weight.stride(0), n, k,
-              group, packed.data_ptr(), scales.data_ptr())
+    with torch.cuda.device(weight.device):
+        _lib.call("hb_quant_w4", weight.data_ptr(), weight.stride(0), n, k, group, packed.data_ptr(),
+                  scales.data_ptr(), stream_handle(weight.device))
     return packed, scales
 
 
@@ -117,11 +121,11 @@ def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, out_f
         bias = bias.contiguous()
     m, k = x.shape
     if out is None:
-        out = torch.empty((m, out_features), dtype=x.dtype, device=x.device)
+        out = x.new_empty((m, out_features))
     if m:
-        launch_on(device, "hb_w4_linear", _lib.lib().hb_w4_linear, x_at, x.stride(0), packed.data_ptr(),
-                  scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0), m,
-                  out_features, k, group, act_code, dtype_code)
+        launch(device, "hb_w4_linear", _lib.lib().hb_w4_linear,
+               _ARGS.pack(x_at, packed.data_ptr(), scales.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                          out.data_ptr(), x.stride(0), out.stride(0), m, out_features, k, group, act_code, dtype_code))
     return out
 
 

@@ -254,15 +254,25 @@ int hb_w8a8_gemm_glu(const void* qx, int64_t ldqx, const float* sx, const void* 
  * No reference counterpart: the reference's conditioning embedders are bf16 `_linear`s (dit.py:33-42). */
 int hb_quant_w4(const void* w, int64_t ldw, int N, int K, int group, void* packed, void* scales, cudaStream_t stream);
 
+/* A call of hb_w4_linear. */
+typedef struct HbW4Args {
+  const void* x;
+  const void* packed;
+  const void* scales;
+  const void* bias;
+  void* y;
+  int64_t ldx, ldy;
+  int M, N, K, group, silu, dtype;
+} HbW4Args;
+
 /* y[m, n] = act(sum_k x[m, k] * q[n, k] * s[n, k / group] + bias[n]) for weights of hb_quant_w4's layout (any q in
  * [-8, 7]); replaces `dit._linear` (dit.py:33-36) where few rows go through it, as in the timestep, global and adaLN
  * embedders (dit.py:39-42), whose SiLU can be taken along.
- *   x [M, K] (ldx elements, rows 16-byte aligned), bias [N] or NULL, y [M, N] (ldy elements): bf16 or fp16 (dtype).
- *   silu  1: act(v) = v / (1 + exp(-v)); 0: none.
+ *   x [M, K] (ldx elements, rows 16-byte aligned), bias [N] or NULL, y [M, N] (ldy elements): bf16 or fp16 (dtype:
+ *   HB_BF16 or HB_FP16). silu 1: act(v) = v / (1 + exp(-v)); 0: none.
  * fp32 sums, one rounding at the end; the same call gives the same bits. Any M is computed; the weights are read once
  * for every 32 rows, so beyond a few dozen rows a W8A8 GEMM is the faster layer. */
-int hb_w4_linear(const void* x, int64_t ldx, const void* packed, const void* scales, const void* bias, void* y,
-                 int64_t ldy, int M, int N, int K, int group, int silu, int dtype, cudaStream_t stream);
+int hb_w4_linear(const HbW4Args* args, cudaStream_t stream);
 
 /* ---- DiT block glue (the elementwise steps around the kernels above) ------------------------------------ */
 /* No reference counterpart as entry points: the reference runs these steps as separate XLA ops inside

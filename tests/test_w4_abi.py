@@ -18,10 +18,11 @@ def lib():
 
 
 def _linear(**kw):
-    a = dict(x=P, ldx=1024, packed=P, scales=P, bias=None, y=P, ldy=6144, m=2, n=6144, k=1024, group=128, silu=0,
-             dtype=_lib.HB_BF16, stream=None)
+    a = dict(x=P, packed=P, scales=P, bias=0, y=P, ldx=1024, ldy=6144, m=2, n=6144, k=1024, group=128, silu=0,
+             dtype=_lib.HB_BF16)
+    assert set(kw) <= set(a)
     a.update(kw)
-    return list(a.values())
+    return w4._ARGS.pack(*(0 if v is None else v for v in a.values())), None
 
 
 @pytest.mark.parametrize("override,status", [
@@ -35,6 +36,11 @@ def _linear(**kw):
 ])
 def test_linear_rejects(lib, override, status):
     assert lib.hb_w4_linear(*_linear(**override)) == status
+
+
+def test_struct_has_the_header_s_size_and_null_is_refused(lib):
+    assert w4._ARGS.size == 5 * 8 + 2 * 8 + 6 * 4
+    assert lib.hb_w4_linear(None, None) == _lib.HB_ERR_NULL
 
 
 @pytest.mark.parametrize("args,status", [
