@@ -12,9 +12,11 @@
 // or-ed into the mantissa of 128 (bf16) or 1024 (fp16) and 136 or 1032 subtracted: q exactly, without a conversion.
 // Each group's sum is accumulated by the MMAs in fp32 and multiplied by its scale once, in fp32.
 //
-// One CTA takes 16 outputs; its eight warps take every eighth block of 128 inputs, each through a ring of asynchronous
-// copies of its own, and merge through shared memory in warp order, so the result does not depend on timing. x is
-// read through L1 (it is the same few rows for every CTA).
+// One CTA takes 16 outputs (or 32); its four warps take every fourth block of 128 inputs, each through a ring of
+// asynchronous copies of its own, and merge through shared memory in warp order, so the result does not depend on
+// timing. x is read through L1 (it is the same few rows for every CTA).
+// One row, 16,384 x 8,192, group 128: 17.8 us, 3.9 TB/s, 59 % of the measured copy rate; unpacking bounds it (the
+// integer pipe is busy half of the time, instruction issue 60 %; 22 us with two logic operations to a nibble pair).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -27,7 +29,7 @@
 namespace hb {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kStages = 4;  // blocks of a warp on their way
 
 struct W4Params {
@@ -41,12 +43,26 @@ struct W4Params {
   int M, N, K, kblocks, silu;
 };
 
+// (a & b) | c as one operation (from the expression the compiler makes two, each with its constant in place).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
 template <bool kFp16>
 struct Half;
 template <>
 struct Half<false> {
-  static __device__ __forceinline__ uint32_t weights(uint32_t w) {  // nibbles 0 and 4 of w
-    const uint32_t u = (w & 0x000f000fu) | 0x43004300u;
+  // The pairs 0 1, 2 3, 4 5, 6 7 of a word's weights.
+  static __device__ __forceinline__ void weights(uint32_t w, uint32_t& p0, uint32_t& p1, uint32_t& p2, uint32_t& p3) {
+    p0 = pair(w);
+    p1 = pair(w >> 4);
+    p2 = pair(w >> 8);
+    p3 = pair(w >> 12);
+  }
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {  // nibbles 0 and 4
+    const uint32_t u = and_or(w, 0x000f000fu, 0x43004300u);
     const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);
     const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), off);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -62,10 +78,23 @@ struct Half<false> {
 };
 template <>
 struct Half<true> {
-  static __device__ __forceinline__ uint32_t weights(uint32_t w) {
-    const uint32_t u = (w & 0x000f000fu) | 0x64006400u;
-    const __half2 off = __floats2half2_rn(1032.f, 1032.f);
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), off);
+  // fp16's mantissa has room for a nibble at bit 4 too: 1024 + 16 u, exactly u - 8 after one FMA.
+  static __device__ __forceinline__ void weights(uint32_t w, uint32_t& p0, uint32_t& p1, uint32_t& p2, uint32_t& p3) {
+    const uint32_t v = w >> 8;
+    p0 = low(w);
+    p1 = high(w);
+    p2 = low(v);
+    p3 = high(v);
+  }
+  static __device__ __forceinline__ uint32_t low(uint32_t w) {
+    const uint32_t u = and_or(w, 0x000f000fu, 0x64006400u);
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1032.f, 1032.f));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ uint32_t high(uint32_t w) {
+    const uint32_t u = and_or(w, 0x00f000f0u, 0x64006400u);
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(0.0625f, 0.0625f),
+                              __floats2half2_rn(-72.f, -72.f));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
   static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -82,109 +111,135 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-template <bool kFp16, int NT, int kGroup>
-__global__ void __launch_bounds__(32 * kWarps) w4_linear_kernel(const W4Params p) {
+// NT: groups of eight rows of x. RT: tiles of 16 outputs that share what a warp reads of x.
+template <bool kFp16, int NT, int RT, int kGroup>
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 8 : NT == 2 ? 4 : 3 - RT / 2) w4_linear_kernel(const W4Params p) {
   using T = Half<kFp16>;
   constexpr int kSteps = kGroup / 32;        // word steps per group
   constexpr int kGroups = 128 / kGroup;      // groups per block
-  constexpr int kStageBytes = 1024 + 32 * kGroups;
+  constexpr int kTileBytes = 1024 + 32 * kGroups, kStageBytes = RT * kTileBytes;
   constexpr int kRing = kStages * kStageBytes;
-  constexpr int kPart = 16 * (8 * NT + 1) * 4;
+  constexpr int kRow = 8 * NT + 1, kPart = RT * 16 * kRow * 4;
   __shared__ __align__(16) uint8_t smem[kWarps * (kRing > kPart ? kRing : kPart)];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
-  const int tile = blockIdx.x, m0 = blockIdx.y * 8 * NT;
+  const int tile = blockIdx.x * RT, m0 = blockIdx.y * 8 * NT;
 
-  float acc[NT][4];
+  float acc[RT][NT][4];
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int q = 0; q < RT; ++q)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[q][t][e] = 0.f;
 
   // Each warp's blocks through a ring of its own: a lane copies what it reads of the weights itself, the scales are
-  // read by all.
-  const uint8_t* wp = reinterpret_cast<const uint8_t*>(p.packed) + (int64_t)tile * p.kblocks * 1024 + lane * 16;
-  const uint8_t* sp = reinterpret_cast<const uint8_t*>(p.scales) + (int64_t)tile * p.kblocks * (32 * kGroups) +
-                      (lane < 2 * kGroups ? lane * 16 : 0);
+  // read by all. The integer pipe bounds this loop (seven operations to a word of eight weights), so all else is kept
+  // off it: pointers that step, stages by unrolling, rows past M read as row M - 1 (their columns are dropped).
+  const uint8_t* wp =
+      reinterpret_cast<const uint8_t*>(p.packed) + ((int64_t)tile * p.kblocks + warp) * 1024 + lane * 16;
+  const uint8_t* sp = reinterpret_cast<const uint8_t*>(p.scales) +
+                      ((int64_t)tile * p.kblocks + warp) * (32 * kGroups) + (lane < 2 * kGroups ? lane * 16 : 0);
   const uint8_t* ring = smem + warp * kRing;
-  const uint32_t ring_at = smem_u32(ring);
-  auto load = [&](int kb, int st) {  // one commit group, also where nothing is copied
-    if (kb < p.kblocks) {
-      const uint32_t dst = ring_at + st * kStageBytes + lane * 16;
-      cp16(dst, wp + (int64_t)kb * 1024);
-      cp16(dst + 512, wp + (int64_t)kb * 1024 + 512);
-      if (lane < 2 * kGroups) cp16(dst + 1024, sp + (int64_t)kb * (32 * kGroups));
+  const uint32_t ring_at = smem_u32(ring) + lane * 16;
+  // (an odd number of tiles: the last one twice, and its second result dropped)
+  const int64_t more_tiles = RT > 1 && (tile + 1) * 16 < p.N ? p.kblocks : 0;
+  const int mine = (p.kblocks - warp + kWarps - 1) / kWarps;  // this warp's blocks
+  auto load = [&](bool more, int st) {  // the next block; one commit group, also where there is none
+    if (more) {
+#pragma unroll
+      for (int q = 0; q < RT; ++q) {
+        const uint32_t dst = ring_at + st * kStageBytes + q * kTileBytes;
+        const uint8_t *w = wp + q * more_tiles * 1024, *s = sp + q * more_tiles * (32 * kGroups);
+        cp16(dst, w);
+        cp16(dst + 512, w + 512);
+        if (lane < 2 * kGroups) cp16(dst + 1024, s);
+      }
+      wp += kWarps * 1024;
+      sp += kWarps * (32 * kGroups);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) load(warp + s * kWarps, s);
+  for (int s = 0; s < kStages - 1; ++s) load(s < mine, s);
 
   const uint16_t* xp[NT];
-  bool live[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int m = m0 + t * 8 + gid;
-    live[t] = m < p.M;
-    xp[t] = p.x + (live[t] ? m : 0) * p.ldx + tid * 8;
-  }
-  int st = 0;
-  for (int kb = warp; kb < p.kblocks; kb += kWarps) {
-    load(kb + (kStages - 1) * kWarps, st == 0 ? kStages - 1 : st - 1);
-    const int k0 = kb * 128;
-    uint4 xv[NT][4];
+  for (int t = 0; t < NT; ++t) xp[t] = p.x + min(m0 + t * 8 + gid, p.M - 1) * p.ldx + warp * 128 + tid * 8;
+  for (int i0 = 0; i0 < mine; i0 += kStages) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int st = 0; st < kStages; ++st) {
+      const int i = i0 + st;
+      if (i >= mine) break;
+      load(i + kStages - 1 < mine, (st + kStages - 1) % kStages);
+      uint4 xv[NT][4];
+      if ((i * kWarps + warp) * 128 + 128 <= p.K) {
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
-        xv[t][w] = live[t] && k0 + 32 * w < p.K ? __ldg(reinterpret_cast<const uint4*>(xp[t] + k0 + 32 * w))
-                                                : make_uint4(0u, 0u, 0u, 0u);
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-    __syncwarp();
-    const uint8_t* stage = ring + st * kStageBytes;
-    const uint4 wa = *reinterpret_cast<const uint4*>(stage + lane * 16);
-    const uint4 wb = *reinterpret_cast<const uint4*>(stage + 512 + lane * 16);
-    const uint32_t lo[4] = {wa.x, wa.y, wa.z, wa.w}, hi[4] = {wb.x, wb.y, wb.z, wb.w};
-    const uint16_t* sc = reinterpret_cast<const uint16_t*>(stage + 1024) + gid;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      float c[NT][4];
+          for (int w = 0; w < 4; ++w) xv[t][w] = __ldg(reinterpret_cast<const uint4*>(xp[t] + 32 * w));
+      } else {  // the row's last block, where K is no multiple of 128
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[t][e] = 0.f;
+          for (int w = 0; w < 4; ++w)
+            xv[t][w] = (i * kWarps + warp) * 128 + 32 * w < p.K ? __ldg(reinterpret_cast<const uint4*>(xp[t] + 32 * w))
+                                                                : make_uint4(0u, 0u, 0u, 0u);
+      }
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int w = g * kSteps + s;
-        const uint32_t a0[4] = {T::weights(lo[w]), T::weights(hi[w]), T::weights(lo[w] >> 4), T::weights(hi[w] >> 4)};
-        const uint32_t a1[4] = {T::weights(lo[w] >> 8), T::weights(hi[w] >> 8), T::weights(lo[w] >> 12),
-                                T::weights(hi[w] >> 12)};
+      for (int t = 0; t < NT; ++t) xp[t] += kWarps * 128;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      __syncwarp();
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          T::mma(c[t], a0, xv[t][w].x, xv[t][w].y);
-          T::mma(c[t], a1, xv[t][w].z, xv[t][w].w);
+      for (int q = 0; q < RT; ++q) {
+        const uint8_t* stage = ring + st * kStageBytes + q * kTileBytes;
+        const uint4 wa = *reinterpret_cast<const uint4*>(stage + lane * 16);
+        const uint4 wb = *reinterpret_cast<const uint4*>(stage + 512 + lane * 16);
+        const uint32_t lo[4] = {wa.x, wa.y, wa.z, wa.w}, hi[4] = {wb.x, wb.y, wb.z, wb.w};
+        const uint16_t* sc = reinterpret_cast<const uint16_t*>(stage + 1024) + gid;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          float c[NT][4];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[t][e] = 0.f;
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            const int w = g * kSteps + s;
+            uint32_t a0[4], a1[4];
+            T::weights(lo[w], a0[0], a0[2], a1[0], a1[2]);
+            T::weights(hi[w], a0[1], a0[3], a1[1], a1[3]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              T::mma(c[t], a0, xv[t][w].x, xv[t][w].y);
+              T::mma(c[t], a1, xv[t][w].z, xv[t][w].w);
+            }
+          }
+          const float s0 = __uint_as_float((uint32_t)sc[g * 16] << 16);
+          const float s1 = __uint_as_float((uint32_t)sc[g * 16 + 8] << 16);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[q][t][e] = fmaf(e < 2 ? s0 : s1, c[t][e], acc[q][t][e]);
         }
       }
-      const float s0 = __uint_as_float((uint32_t)sc[g * 16] << 16), s1 = __uint_as_float((uint32_t)sc[g * 16 + 8] << 16);
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(e < 2 ? s0 : s1, c[t][e], acc[t][e]);
+      __syncwarp();  // every lane has read the stage's scales before it is filled again
     }
-    __syncwarp();  // every lane has read the stage's scales before it is filled again
-    if (++st == kStages) st = 0;
   }
   __syncthreads();  // (the copies still in flight are empty groups) the rings become the partial sums
   float* part = reinterpret_cast<float*>(smem);
-  constexpr int kRow = 8 * NT + 1, kWarp = 16 * kRow;
+  constexpr int kWarp = RT * 16 * kRow;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int q = 0; q < RT; ++q)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      part[warp * kWarp + (gid + 8 * (e >> 1)) * kRow + t * 8 + tid * 2 + (e & 1)] = acc[t][e];
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        part[warp * kWarp + (q * 16 + gid + 8 * (e >> 1)) * kRow + t * 8 + tid * 2 + (e & 1)] = acc[q][t][e];
   __syncthreads();
   const int warps = min(kWarps, p.kblocks);
-  for (int i = threadIdx.x; i < 128 * NT; i += 32 * kWarps) {
-    const int r = i & 15, c = i >> 4, n = tile * 16 + r, m = m0 + c;
+  for (int i = threadIdx.x; i < RT * 128 * NT; i += 32 * kWarps) {
+    const int r = i % (16 * RT), c = i / (16 * RT), n = tile * 16 + r, m = m0 + c;
     if (n >= p.N || m >= p.M) continue;
     float v = part[r * kRow + c];
     for (int w = 1; w < warps; ++w) v += part[w * kWarp + r * kRow + c];
@@ -236,17 +291,22 @@ __global__ void __launch_bounds__(256) w4_quant_kernel(const uint16_t* __restric
         live ? __bfloat16_as_ushort(__float2bfloat16_rn(s)) : 0;
 }
 
-template <bool kFp16, int NT>
-void launch_linear(const W4Params& p, int group, dim3 grid, cudaStream_t s) {
-  if (group == 32) w4_linear_kernel<kFp16, NT, 32><<<grid, 32 * kWarps, 0, s>>>(p);
-  if (group == 64) w4_linear_kernel<kFp16, NT, 64><<<grid, 32 * kWarps, 0, s>>>(p);
-  if (group == 128) w4_linear_kernel<kFp16, NT, 128><<<grid, 32 * kWarps, 0, s>>>(p);
+template <bool kFp16, int NT, int RT>
+void launch_linear(const W4Params& p, int group, cudaStream_t s) {
+  const dim3 grid((p.N + 16 * RT - 1) / (16 * RT), (p.M + 8 * NT - 1) / (8 * NT));
+  if (group == 32) w4_linear_kernel<kFp16, NT, RT, 32><<<grid, 32 * kWarps, 0, s>>>(p);
+  if (group == 64) w4_linear_kernel<kFp16, NT, RT, 64><<<grid, 32 * kWarps, 0, s>>>(p);
+  if (group == 128) w4_linear_kernel<kFp16, NT, RT, 128><<<grid, 32 * kWarps, 0, s>>>(p);
 }
 template <bool kFp16>
-void launch_linear(const W4Params& p, int nt, int group, dim3 grid, cudaStream_t s) {
-  if (nt == 1) launch_linear<kFp16, 1>(p, group, grid, s);
-  if (nt == 2) launch_linear<kFp16, 2>(p, group, grid, s);
-  if (nt == 4) launch_linear<kFp16, 4>(p, group, grid, s);
+void launch_linear(const W4Params& p, int group, cudaStream_t s) {
+  // Two tiles to a CTA halve the reads of x, at half the CTAs: worth it where x is more than L1 keeps beside the rings
+  // and the CTAs still fill the GPU (16,384 x 8,192: 16 rows 36.8 -> 25.2 us, 32 rows 59.9 -> 46.0; below that
+  // slower: 8,201 x 4,096, 13 rows 9.1 -> 9.9 us, 2,000 x 4,096 5.9 -> 7.8).
+  const bool wide = (int64_t)p.M * p.K * 2 > 160 * 1024 && p.N > 2 * 148 * 16;
+  if (p.M <= 8) return launch_linear<kFp16, 1, 1>(p, group, s);
+  if (p.M <= 16) return wide ? launch_linear<kFp16, 2, 2>(p, group, s) : launch_linear<kFp16, 2, 1>(p, group, s);
+  return wide ? launch_linear<kFp16, 4, 2>(p, group, s) : launch_linear<kFp16, 4, 1>(p, group, s);
 }
 
 bool w4_shape_ok(int N, int K, int group) {
@@ -303,11 +363,9 @@ extern "C" int hb_w4_linear(const HbW4Args* args, cudaStream_t stream) {
                    a.K,
                    (a.K + 127) / 128,
                    a.silu};
-  const int nt = a.M <= 8 ? 1 : a.M <= 16 ? 2 : 4;
-  const dim3 grid((a.N + 15) / 16, (a.M + 8 * nt - 1) / (8 * nt));
   if (a.dtype == HB_FP16)
-    launch_linear<true>(p, nt, a.group, grid, stream);
+    launch_linear<true>(p, a.group, stream);
   else
-    launch_linear<false>(p, nt, a.group, grid, stream);
+    launch_linear<false>(p, a.group, stream);
   return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
