@@ -4,8 +4,6 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
-#include "hb_status.h"
-
 namespace hb {
 
 // Division of n < 2^31 by a fixed d >= 1: q = umulhi(n, ceil(2^p / d)) >> (p - 32) with p = 31 + ceil(log2 d), exact
@@ -122,25 +120,6 @@ constexpr int ctx_tile_keys(int D) { return D == 64 ? 64 : 128; }
 constexpr int ctx_tile_ctas(int D) { return (D == 64 ? 4 : 2) * kCtxSms; }
 // Mask bits of a unit's keys are kept in shared memory, for at most this many tiles.
 constexpr int kCtxMaskTiles = 256;
-
-// Launch a kernel that may begin while the one before it in the stream still runs (that one lets it, by
-// griddepcontrol.launch_dependents, once all its CTAs have started). A kernel launched so waits for the one before
-// (griddepcontrol.wait) before it reads its results, and before it ends, so that whoever waits for it has both.
-template <class... P, class... A>
-int ctx_launch_after(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
-                     const A&... args) {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
-}
 
 // Launchers of the parts whose `count` is not 0: a CUDA error (or a kernel that cannot be launched) returns
 // HB_ERR_LAUNCH. The few-rows kernel (context_rows.cu; rows_per_tile 16, or 32 at D 64), the tcgen05 kernel on

@@ -17,6 +17,7 @@
 
 #include "context_attn.h"
 #include "hb_sm100.cuh"
+#include "launch_after.h"
 
 namespace hb {
 namespace {
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
   uint32_t* bits_s = reinterpret_cast<uint32_t*>(smem + kWarps * kWarpBytes);
   float2* ml_s = reinterpret_cast<float2*>(smem + kWarps * kWarpBytes + kWarps * kStages * 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tid = lane & 3;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the tcgen05 kernel beside it, or the merge
+  wait_for_kernel_before();
 
   // ---- which item
   const bool second = static_cast<int>(blockIdx.x) >= p.part[0].count;
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
 template <int D, class T, int kTeams>
 __global__ void __launch_bounds__(256) ctx_combine_kernel(const CtxParams p) {
   constexpr int TPR = D / 4;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the partial results of every kernel of this call
+  wait_for_kernel_before();  // the partial results of every kernel of this call
   __shared__ float4 acc_s[256];
   __shared__ float2 ml_s[256];
   const int idx = static_cast<int>(((int64_t)blockIdx.x * 256 + threadIdx.x) / TPR);
@@ -424,14 +425,13 @@ int launch_rows(const CtxParams& p, cudaStream_t s) {
       return HB_ERR_LAUNCH;
     if (dev < 64) configured[dev] = true;
   }
-  ctx_rows_kernel<D, T, MT><<<p.part[0].count + p.part[1].count, 32 * kWarps, kRowsSmem, s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
+  return launch_after(false, ctx_rows_kernel<D, T, MT>, p.part[0].count + p.part[1].count, 32 * kWarps, kRowsSmem, s, p);
 }
 
 template <int D, class T, int kTeams>
 int launch_teams(const CtxParams& p, cudaStream_t s) {
   const int64_t threads = (int64_t)p.prows * (D / 4) * kTeams;
-  return ctx_launch_after(ctx_combine_kernel<D, T, kTeams>, static_cast<unsigned>((threads + 255) / 256), 256, 0, s, p);
+  return launch_after(true, ctx_combine_kernel<D, T, kTeams>, static_cast<unsigned>((threads + 255) / 256), 256, 0, s, p);
 }
 // As many teams as it takes to have about a thousand threads on every SM, and no more than have slots to read.
 template <int D, class T>

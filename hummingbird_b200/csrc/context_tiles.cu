@@ -29,6 +29,7 @@
 #include <cudaTypedefs.h>
 
 #include "context_attn.h"
+#include "launch_after.h"
 #include "hb_sm100.cuh"
 
 namespace hb {
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
   uint32_t* bits0 = reinterpret_cast<uint32_t*>(smem + L::kOffBits);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge, which waits for this kernel
   const int count0 = p.part[0].count, total = count0 + p.part[1].count;
 
   if (warp == 4 && lane == 0) {
@@ -612,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
     tc_fence_after();
     tmem_dealloc(tmem, L::kTmemCols);
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the few-rows kernel, where this one was launched beside it
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the few-rows kernel, where this one runs beside it
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -661,9 +662,7 @@ int launch_tiles(const CUtensorMap& own, const CUtensorMap& shared, const CtxPar
     if (dev < 64) configured[dev] = true;
   }
   const int grid = std::min(p.part[0].count + p.part[1].count, ctx_tile_ctas(D));
-  if (beside) return ctx_launch_after(kernel, grid, kThreads, Layout<D>::bytes(mask_tiles), s, own, shared, p, mask_tiles);
-  kernel<<<grid, kThreads, Layout<D>::bytes(mask_tiles), s>>>(own, shared, p, mask_tiles);
-  return cudaGetLastError() == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
+  return launch_after(beside, kernel, grid, kThreads, Layout<D>::bytes(mask_tiles), s, own, shared, p, mask_tiles);
 }
 
 template <int D, bool kFp16>
