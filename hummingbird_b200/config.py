@@ -3,7 +3,8 @@
 `sa3jax.config.DiTConfig.attention` is `"xla" | "fused"` (config.py:57) and `SameConfig.attention` is
 `"xla" | "pallas"` (config.py:115); both fall back to XLA off TPU. Here `"cuda"` selects the sm_100a kernels,
 and a new `DiTConfig.ff_quant = "w8a8"` selects the W8A8 MLP (the reference has no int8 role,
-dtypes.py:23-37). Only the fields the hot paths read are mirrored; the shapes follow the reference's
+dtypes.py:23-37), `cond_quant = "w4"` 4-bit conditioning embedders and `cross_differential = False` the plain
+cross-attention. Only the fields the hot paths read are mirrored; the shapes follow the reference's
 properties (`head_dim`, `rope_dim`, `sub_chunk_size`).
 """
 from __future__ import annotations
@@ -34,6 +35,12 @@ class DiTConfig:
     # "w8a8": the self-attention's `to_out` as a W8A8 GEMM; its input (the attention output, written per head by
     # the attention kernel) is quantised per token by a separate quantiser pass (glue="cuda")
     out_quant: Literal["none", "w8a8"] = "none"
+    # False: plain cross-attention (`SDPA(q, k, v)`, the reference's presets without the differential branch) over
+    # the context, with a padding mask and, optionally, states that every clip of the batch shares
+    cross_differential: bool = True
+    cross_kv_heads: int | None = None  # kv heads of the plain cross-attention (None: num_heads)
+    # "w4": the timestep, global and adaLN embedders (one row per clip) as 4-bit weights with group scales
+    cond_quant: Literal["none", "w4"] = "none"
     full_head_rope: bool = False  # True: rotate all 64 dims (the benchmark configs); False: the reference's 32
 
     @property
@@ -44,6 +51,10 @@ class DiTConfig:
     def rope_dim(self) -> int:
         """`RotaryEmbedding(max(dim_heads // 2, 32))` (config.py:67-70), or the full head."""
         return self.head_dim if self.full_head_rope else max(self.head_dim // 2, 32)
+
+    @property
+    def context_kv_heads(self) -> int:
+        return self.num_heads if self.cross_kv_heads is None else self.cross_kv_heads
 
     @property
     def ff_inner(self) -> int:

@@ -3,9 +3,12 @@
 Used to time a whole 120 s clip (the benchmark's config 4): `sa3jax.sampling.pingpong` (sampling.py:81-118)
 over `sa3jax.dit.dit_forward` (dit.py:340-361) with its 24 `_block`s (dit.py:224-250). The self-attention is
 this library's fused differential kernel (`blocks.dit_self_attention`'s path); the MLP is W8A8 when
-`DiTConfig.ff_quant == "w8a8"` (else a bf16 matmul); with `glue="cuda"` the differential cross-attention over
+`DiTConfig.ff_quant == "w8a8"` (else a bf16 matmul); the timestep, global and adaLN embedders are 4-bit linears when
+`DiTConfig.cond_quant == "w4"`; with `glue="cuda"` the differential cross-attention over
 the 128 hoisted context tokens (dit.py:203-215, 274-284) is this library's `hb_cross_diff_attn` kernel and the
-residual / RMSNorm / adaLN / GLU steps its row kernels; projections are torch matmuls (cuBLAS). With
+residual / RMSNorm / adaLN / GLU steps its row kernels; with `DiTConfig.cross_differential` off the cross-attention is
+`hb_context_attn` over a padded context and, where `prepare_static` is given them, states that all clips share;
+projections are torch matmuls (cuBLAS). With
 `glue="torch"` the cross-attention and the elementwise steps run as torch ops (cuDNN-flash SDPA). No checkpoint
 is loaded: weights are N(0, 1 / fan_in) bf16 draws.
 
@@ -30,11 +33,13 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
+from hummingbird_b200 import context_attention as hb_context
 from hummingbird_b200 import cross_attention as hb_cross
 from hummingbird_b200 import dense_attention as hb_dense
 from hummingbird_b200 import dit_glue as glue
 from hummingbird_b200 import parallel as par
 from hummingbird_b200.config import DiTConfig
+from hummingbird_b200.w4 import W4Linear
 from hummingbird_b200.w8a8 import W8A8GluLinear, W8A8Linear, quantize_rows, w8a8_gemm
 
 
@@ -110,6 +115,8 @@ class DiT:
             raise ValueError("qkv_quant='w8a8' needs glue='cuda' and one rank per batch group")
         if cfg.out_quant == "w8a8" and glue != "cuda":
             raise ValueError("out_quant='w8a8' needs glue='cuda'")
+        if cfg.num_heads % cfg.context_kv_heads or (cfg.cross_differential and cfg.cross_kv_heads is not None):
+            raise ValueError("cross_kv_heads must divide num_heads and needs cross_differential=False")
         if (cfg.num_heads // 2) % self.world or self.t1 - self.t0 <= self.mem_rows:
             raise ValueError(f"a clip of {self.seq} tokens and {cfg.num_heads // 2} head pairs does not split "
                              f"over {self.world} ranks (equal pair counts, latent rows on every rank)")
@@ -127,6 +134,12 @@ class DiT:
             "rope_inv_freq": (1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.rope_dim, 2, device=device).float()
                                                           / cfg.rope_dim))),
         }
+        # embedders of one row per clip, as `self._embed` runs them
+        self.cond_layers = {name: self.p[name] for name in ("to_global_embed", "to_timestep_embed",
+                                                            "global_cond_embedder")}
+        if cfg.cond_quant == "w4":
+            self.cond_layers = {name: [W4Linear(layers[0], act="silu"), W4Linear(layers[1])]
+                                for name, layers in self.cond_layers.items()}
         self.blocks = []
         for _ in range(shape.depth):
             b = {
@@ -137,7 +150,9 @@ class DiT:
                 "self_attn": {"to_qkv": _w((5 * d, d), g, device), "to_out": _w((d, d), g, device),
                               "q_norm": 1 + 0.02 * torch.randn(cfg.head_dim, generator=g, device=device),
                               "k_norm": 1 + 0.02 * torch.randn(cfg.head_dim, generator=g, device=device)},
-                "cross_attn": {"to_q": _w((2 * d, d), g, device), "to_kv": _w((3 * d, d), g, device),
+                "cross_attn": {"to_q": _w(((2 if cfg.cross_differential else 1) * d, d), g, device),
+                               "to_kv": _w((3 * d if cfg.cross_differential else
+                                            2 * cfg.context_kv_heads * cfg.head_dim, d), g, device),
                                "to_out": _w((d, d), g, device),
                                "q_norm": 1 + 0.02 * torch.randn(cfg.head_dim, generator=g, device=device),
                                "k_norm": 1 + 0.02 * torch.randn(cfg.head_dim, generator=g, device=device)},
@@ -165,10 +180,17 @@ class DiT:
             self.blocks.append(b)
 
     # ------------------------------------------------------------------ per clip
-    def prepare_static(self, cross_cond: torch.Tensor, global_cond: torch.Tensor) -> dict:
+    def prepare_static(self, cross_cond: torch.Tensor, global_cond: torch.Tensor,
+                       cross_mask: torch.Tensor | None = None, shared_cond: torch.Tensor | None = None) -> dict:
         """`dit.prepare_static` (dit.py:287-337): hoisted, k-normed cross K/V per block, conditioning, tables.
-        The conditioning may hold the whole clip's batch rows; this rank's are taken."""
+        The conditioning may hold the whole clip's batch rows; this rank's are taken. With
+        `cross_differential=False`, `cross_mask` `(B, context)` says which context tokens are not padding, and
+        `shared_cond` `(Ls, context_dim)` are states that every clip attends to in front of its own."""
         cross_cond, global_cond = self._rows(cross_cond), self._rows(global_cond)
+        if self.cfg.cross_differential and (cross_mask is not None or shared_cond is not None):
+            raise ValueError("cross_mask and shared_cond need cross_differential=False")
+        if cross_mask is not None:
+            cross_mask = self._rows(cross_mask)
         cfg, d, h = self.cfg, self.cfg.embed_dim, self.cfg.num_heads
         seq = cfg.num_memory_tokens + self.shape.latents
         valid = torch.ones(self.shape.batch, seq, device=self.device)
@@ -178,18 +200,38 @@ class DiT:
         for b in self.blocks:
             x = ctx @ b["cross_attn"]["to_kv"].T
             kn = b["cross_attn"]["k_norm"]
+            if not cfg.cross_differential:
+                kv_rows.append(self._norm_keys(x, kn))
+                continue
             if self.glue == "cuda":  # the kernel's layout: (B, context, [k | k_diff | v]) rows, keys k-normed
                 kv_rows.append(hb_cross.cross_kv(x, kn, h, cfg.qk_norm_eps, cfg.head_dim))
                 continue
             k, kd, v = (t.unflatten(-1, (h, cfg.head_dim)).transpose(1, 2) for t in x.chunk(3, -1))
             kv.append((_rms(k, kn, cfg.qk_norm_eps), _rms(kd, kn, cfg.qk_norm_eps), v))
+        shared_rows = [None] * len(self.blocks)
+        if shared_cond is not None:
+            states = self._seq(self.p["to_cond_embed"], shared_cond.to(torch.bfloat16))
+            shared_rows = [self._norm_keys(states @ b["cross_attn"]["to_kv"].T, b["cross_attn"]["k_norm"])
+                           for b in self.blocks]
         return {"lane_cos": cos, "lane_sin": sin, "lane_mask": mask, "cross_kv": kv, "cross_kv_rows": kv_rows,
-                "gcond_proj": self._seq(self.p["to_global_embed"], global_cond.to(torch.bfloat16))}
+                "cross_mask": cross_mask, "shared_kv_rows": shared_rows,
+                "gcond_proj": self._embed("to_global_embed", global_cond.to(torch.bfloat16))}
+
+    def _norm_keys(self, kv: torch.Tensor, k_weight: torch.Tensor) -> torch.Tensor:
+        """`(..., [k | v])` rows of the plain cross-attention with k RMS-normed per head (dit.py:122-128, 274-284)."""
+        width = self.cfg.context_kv_heads * self.cfg.head_dim
+        k = kv[..., :width].unflatten(-1, (-1, self.cfg.head_dim))
+        return torch.cat([_rms(k, k_weight, self.cfg.qk_norm_eps).flatten(-2), kv[..., width:]], -1).contiguous()
 
     @staticmethod
     def _seq(layers, x):
         """`nn.Sequential(Linear, SiLU, Linear)` without biases (dit.py:39-42)."""
         return F.silu(x @ layers[0].T) @ layers[1].T
+
+    def _embed(self, name: str, x: torch.Tensor) -> torch.Tensor:
+        """`_seq` of a conditioning embedder, in bf16 or on 4-bit weights (`cond_quant`)."""
+        layers = self.cond_layers[name]
+        return layers[1](layers[0](x)) if self.cfg.cond_quant == "w4" else self._seq(layers, x)
 
     # ------------------------------------------------------------------ sharding
     def latent_range(self) -> tuple[int, int]:
@@ -240,8 +282,8 @@ class DiT:
         if self.mem_rows:
             mem = p["memory_tokens"][self.t0:self.t0 + self.mem_rows].expand(h.shape[0], -1, -1)
             h = torch.cat([mem, h], 1)
-        temb = self._seq(p["to_timestep_embed"], _expo_fourier(t.to(torch.bfloat16), cfg.fourier_dim))
-        gcond = self._seq(p["global_cond_embedder"], static["gcond_proj"] + temb)
+        temb = self._embed("to_timestep_embed", _expo_fourier(t.to(torch.bfloat16), cfg.fourier_dim))
+        gcond = self._embed("global_cond_embedder", static["gcond_proj"] + temb)
         if self.glue == "cuda":
             h = self._blocks_fused(h.contiguous(), static, gcond)
         else:
@@ -260,7 +302,10 @@ class DiT:
         h = torch.addcmul(h, self._self_attn(x, b["self_attn"], static) @ b["self_attn"]["to_out"].T,
                           torch.sigmoid(1 - gs))
         x = F.rms_norm(h, (d,), b["cross_attend_norm_bf"], cfg.norm_eps)
-        h = h + self._cross(x, b["cross_attn"], static["cross_kv"][index])
+        if cfg.cross_differential:
+            h = h + self._cross(x, b["cross_attn"], static["cross_kv"][index])
+        else:
+            h = h + self._context(x, b["cross_attn"], static, index)
         h[:, self.mem_rows:] += b["local"]
         x = torch.addcmul(shf, F.rms_norm(h, (d,), b["ff_norm_bf"], cfg.norm_eps), 1 + sf)
         return torch.addcmul(h, self._ff(x, b), torch.sigmoid(1 - gf))
@@ -283,7 +328,10 @@ class DiT:
             c = conds[i]
             y = self._to_out(self._self_attn(x, b["self_attn"], static, lead=h.shape[:-1]), b["self_attn"])
             x = glue.residual_norm(h, y=y, gate=part(c, 2), weight=b["cross_attend_norm_bf"], eps=eps)
-            y = self._cross_fused(x, b["cross_attn"], static["cross_kv_rows"][i])
+            if cfg.cross_differential:
+                y = self._cross_fused(x, b["cross_attn"], static["cross_kv_rows"][i])
+            else:
+                y = self._context_fused(x, b["cross_attn"], static, i)
             if self.cfg.ff_quant == "w8a8":  # the MLP's input leaves the norm kernel already quantised per token
                 qx, sx = glue.residual_norm(h, y=y, local=b["local"], local_row0=self.mem_rows,
                                             weight=b["ff_norm_bf"], scale=part(c, 3), shift=part(c, 4), eps=eps,
@@ -337,6 +385,37 @@ class DiT:
         att = hb_cross.cross_attention(x @ ca["to_q"].T, kv_rows, ca["q_norm_f"], None, cfg.num_heads,
                                        cfg.head_dim, cfg.qk_norm_eps)
         return att @ ca["to_out"].T
+
+    def _context_fused(self, x, ca, static, index):
+        """Plain cross-attention (dit.py:131-147, 203-215 without the differential branch) as this library's kernel:
+        `to_q`, then q RMSNorm and one softmax over the shared states and the clip's own context, then `to_out`."""
+        cfg = self.cfg
+        q, kv, shared = x @ ca["to_q"].T, static["cross_kv_rows"][index], static["shared_kv_rows"][index]
+        args = dict(kv_heads=cfg.context_kv_heads, mask=static["cross_mask"], q_weight=ca["q_norm_f"],
+                    eps=cfg.qk_norm_eps)
+        if shared is None:
+            att = hb_context.context_attention(q, kv, cfg.num_heads, cfg.head_dim, **args)
+        else:
+            att = hb_context.shared_context_attention(q, shared, kv, cfg.num_heads, cfg.head_dim, **args)
+        return att @ ca["to_out"].T
+
+    def _context(self, x, ca, static, index):
+        """`_context_fused` in torch ops."""
+        cfg = self.cfg
+        bsz, length, _ = x.shape
+        q = F.rms_norm((x @ ca["to_q"].T).view(bsz, length, cfg.num_heads, cfg.head_dim), (cfg.head_dim,),
+                       ca["q_norm_bf"], cfg.qk_norm_eps).transpose(1, 2)
+        rows, shared, mask = static["cross_kv_rows"][index], static["shared_kv_rows"][index], static["cross_mask"]
+        if mask is None:
+            mask = torch.ones(rows.shape[:2], dtype=torch.bool, device=x.device)
+        if shared is not None:
+            rows = torch.cat([shared.expand(bsz, -1, -1), rows], 1)
+            mask = torch.cat([mask.new_ones(bsz, shared.shape[0]), mask], 1)
+        k, v = (t.unflatten(-1, (cfg.context_kv_heads, cfg.head_dim)).transpose(1, 2)
+                .repeat_interleave(cfg.num_heads // cfg.context_kv_heads, 1) for t in rows.chunk(2, -1))
+        out = F.scaled_dot_product_attention(q, k, v, attn_mask=mask[:, None, None, :])
+        out = torch.where(mask.any(1)[:, None, None, None], out, torch.zeros_like(out))
+        return out.transpose(1, 2).reshape(bsz, length, -1) @ ca["to_out"].T
 
     def _cross(self, x, ca, kv):
         """Differential cross-attention, no RoPE, no mask (dit.py:203-215): SDPA(q) - SDPA(q_diff), torch ops."""
