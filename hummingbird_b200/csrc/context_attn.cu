@@ -71,7 +71,7 @@ Plan make_plan(const Shape& s) {
     part.use_own = own;
     part.row_tiles = ceil_div(part_rows, tiles ? 128 : p.rows_per_tile);
     const int64_t items = (int64_t)(pool ? 1 : s.B) * s.Hkv * part.row_tiles;
-    const int keys = tiles ? ctx_tile_keys(s.D) : 2048 / s.D, ctas = tiles ? ctx_tile_ctas(s.D) : kCtxRowCtas;
+    const int keys = tiles ? kCtxTileKeys : 2048 / s.D, ctas = tiles ? ctx_tile_ctas(s.D) : kCtxRowCtas;
     const int chunks = (sh ? ceil_div(s.Ls, keys) : 0) + (own ? ceil_div(s.Lkv, keys) : 0);
     // Few items: the key list is cut so that one round of CTAs fills the GPU, down to 256 keys (or two chunks
     // for each of the four warps) per CTA; the merge then costs less than the idle SMs.

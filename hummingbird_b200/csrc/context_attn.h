@@ -116,7 +116,7 @@ __device__ __forceinline__ int ctx_own_len(const CtxParams& p, int b) {
 constexpr int kCtxSms = 148;
 constexpr int kCtxRowCtas = 2 * kCtxSms;  // CTAs of the few-rows kernel that run at once
 // The tcgen05 kernel: keys of a tile, and CTAs that run at once (as many per SM as TMEM holds their S and O for).
-constexpr int ctx_tile_keys(int D) { return D == 64 ? 64 : 128; }
+constexpr int kCtxTileKeys = 64;
 constexpr int ctx_tile_ctas(int D) { return (D == 64 ? 4 : 2) * kCtxSms; }
 // Mask bits of a unit's keys are kept in shared memory, for at most this many tiles.
 constexpr int kCtxMaskTiles = 256;

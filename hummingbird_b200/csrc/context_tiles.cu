@@ -4,11 +4,12 @@
 // S = Q K^T (fp32, TMEM), P = exp2(c S - m) (16-bit, over S in TMEM), O += P V (fp32, TMEM), with the running maximum
 // m and sum of each row in the registers of one thread. The softmax's arithmetic bounds it: maxima, FMAs,
 // exponentials and conversions of 128 scores a row take 980 cycles of an SM with four warps on each of its
-// sub-partitions (1,170 a warp with two, 1,520 with one; measured without any memory or MMA), the MMAs of a tile 660
-// at D 64; and within a tile S, softmax and P V wait for one another, about as long again. So as many CTAs as TMEM
-// holds share an SM and fill each other's waits: at D 64 four, on tiles of 64 keys (S 64 columns, O 64), at D 128 two,
-// on tiles of 128 keys (S 128, O 128). A lazy maximum (O is rescaled only when a row's maximum grows by more than 2^8)
-// keeps O in TMEM, and a share of the exponentials goes to the FMA pipe (exp2_poly2).
+// sub-partitions (1,170 a warp with two, 1,520 with one; measured without any memory or MMA), the MMAs of as many
+// scores 660 to 800 at D 64; and within a tile S, softmax and P V wait for one another, about as long again. So at D 64
+// four CTAs share an SM, as many as TMEM holds their S and O for (64 + 64 columns), and fill each other's waits. At
+// D 128 there is room for two, each with two buffers of S (2 x 64 + 128 columns): the next tile's S runs while this
+// one's softmax does. A lazy maximum (O is rescaled only when a row's maximum grows by more than 2^8) keeps O in
+// TMEM, and a share of the exponentials goes to the FMA pipe (exp2_poly2).
 //
 // The grid is one round of CTAs; each walks its share of the units (tiles of rows), so barriers, TMEM and tensor maps
 // are set up once, K and V of the next unit are on their way early and its queries during the epilogue.
@@ -42,21 +43,23 @@ constexpr int kCtxPolyMask = 3;                  // key pairs j with (j & 3) == 
 
 template <int D>
 struct Layout {
-  static constexpr int kKeys = ctx_tile_keys(D);            // of a tile
+  static constexpr int kKeys = kCtxTileKeys;                // of a tile
   static constexpr int kWords = kKeys / 32;                 // of a tile's mask bits
   static constexpr int kCtasPerSm = ctx_tile_ctas(D) / kCtxSms;
   static constexpr int kLaunchRegs = 256 / kCtasPerSm;      // x 256 threads x kCtasPerSm = the SM's 65,536
   static constexpr int kSoftmaxRegs = D == 64 ? 88 : 184, kOtherRegs = 2 * kLaunchRegs - kSoftmaxRegs;
-  static constexpr int kTmemCols = 512 / kCtasPerSm;        // S (and P) at 0, O at kKeys
-  static_assert(kKeys + D <= kTmemCols, "TMEM columns");
+  static constexpr int kTmemCols = 512 / kCtasPerSm;
+  static constexpr int kScores = D == 64 ? 1 : 2;           // buffers of S (and P) at 0, then O
+  static constexpr int kTmemO = kScores * kKeys;
+  static_assert(kTmemO + D <= kTmemCols, "TMEM columns");
   static constexpr int kHalves = D / 64;
   static constexpr int kAtom = kKeys * 128;                 // 64 columns of a K or V tile
   static constexpr int kTile = kHalves * kAtom;
-  static constexpr int kStages = D == 64 ? 2 : 1;
+  static constexpr int kStages = 2;
   static constexpr int kOffK = kHalves * kQAtom;            // queries at 0
   static constexpr int kOffV = kOffK + kStages * kTile;
   static constexpr int kOffBars = kOffV + kStages * kTile;
-  static constexpr int kBars = 4 * kStages + 9;
+  static constexpr int kBars = 4 * kStages + 10;
   static constexpr int kOffMisc = kOffBars + kBars * 8;     // TMEM address, abort flag
   static constexpr int kOffBits = (kOffMisc + 8 + 15) & ~15;
   static constexpr int bytes(int mask_tiles) { return kOffBits + 2 * mask_tiles * kWords * 4 + 1024; }
@@ -206,9 +209,9 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
   uint64_t* v_full = k_empty + kStages;     // [kStages] TMA bytes
   uint64_t* v_empty = v_full + kStages;     // [kStages] commit of the P V MMAs
   uint64_t* q_full = v_empty + kStages;     // 4 softmax warps wrote the queries (units that have keys)
-  uint64_t* s_full = q_full + 1;            // commit: S written
-  uint64_t* p_ready = s_full + 1;           // 4 softmax warps wrote P
-  uint64_t* o_done = p_ready + 1;           // commit: the unit's last P V added
+  uint64_t* s_full = q_full + 1;            // [kScores] commit: S written
+  uint64_t* p_ready = s_full + 2;           // 4 softmax warps wrote P
+  uint64_t* o_done = p_ready + 1;           // commit: P V added (one S buffer: the unit's last)
   uint64_t* drain = o_done + 1;
   uint64_t* m_full = drain + 1;             // [2] warp 6 wrote the unit's mask bits
   uint64_t* m_free = m_full + 2;            // [2] the six roles' warps are through with them
@@ -229,7 +232,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
       mbar_init(&v_empty[i], 1);
     }
     mbar_init(q_full, 4);
-    mbar_init(s_full, 1);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
     mbar_init(p_ready, 4);
     mbar_init(o_done, 1);
     mbar_init(drain, 1);
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
       const uint64_t dk = smem_desc_sw128(smem_u32(smem + L::kOffK));
       // V tiles are MN-major: 16 keys are 2,048 bytes on, the second 64 columns one atom on
       const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kOffV), D == 64 ? 16 : L::kAtom);
-      const uint32_t tS = tmem, tO = tmem + kKeys;
+      const uint32_t tO = tmem + L::kTmemO;
       int it = 0, units = 0;
       auto issue_s = [&](int i, int n16) {
         const int st = i % kStages;
@@ -337,9 +341,9 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const int half = k / 4, at = (k % 4) * 32;
-          mma_ss(lead, tS, dq + ((half * kQAtom + at) >> 4), kd + ((half * L::kAtom + at) >> 4), id, k > 0);
+          mma_ss(lead, tmem + i % L::kScores * kKeys, dq + ((half * kQAtom + at) >> 4), kd + ((half * L::kAtom + at) >> 4), id, k > 0);
         }
-        commit(lead, s_full);
+        commit(lead, &s_full[i % L::kScores]);
         commit(lead, &k_empty[st]);
         return true;
       };
@@ -362,17 +366,19 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
         if (j < ks.j1) ok = warp_wait(q_full, units++ & 1, abort_flag) && issue_s(it, n16);
         for (bool first = true; ok && j < ks.j1; first = false) {
           const int jn = next_tile(j + 1, n16_next), st = it % kStages;
+          // two buffers: the next S while the softmax computes this tile's P
+          if (L::kScores == 2 && jn < ks.j1 && !(ok = issue_s(it + 1, n16_next))) break;
           if (!(ok = warp_wait(&v_full[st], (it / kStages) & 1, abort_flag) && warp_wait(p_ready, it & 1, abort_flag)))
             break;
           tc_fence_after();
           const uint64_t vd = dv + st * (L::kTile >> 4);
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)
-            if (16 * k < n16) mma_ts(lead, tO, tS + 8 * k, vd + k * (2048 >> 4), idO, !first || k > 0);
-          if (jn >= ks.j1) commit(lead, o_done);
+            if (16 * k < n16) mma_ts(lead, tO, tmem + it % L::kScores * kKeys + 8 * k, vd + k * (2048 >> 4), idO, !first || k > 0);
+          if (L::kScores == 2 || jn >= ks.j1) commit(lead, o_done);
           commit(lead, &v_empty[st]);
-          // in the tensor pipe's order: P V reads P before the next S overwrites it
-          if (jn < ks.j1 && !(ok = issue_s(it + 1, n16_next))) break;
+          // one: in the tensor pipe's order, P V reads P before the next S overwrites it
+          if (L::kScores == 1 && jn < ks.j1 && !(ok = issue_s(it + 1, n16_next))) break;
           ++it;
           j = jn;
           n16 = n16_next;
@@ -411,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftmaxRegs));
     const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
-    const uint32_t tS = tmem + lane_base, tO = tS + kKeys;
+    const uint32_t tO = tmem + lane_base + L::kTmemO;
     const int row = warp * 32 + lane;
     int it = 0, done = 0;
     bool ok = true;
@@ -457,8 +463,9 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
         const Tile<kKeys> t = tile_of<kKeys, kMask>(p, ks, j, bits);
         if (t.hi <= 0) continue;
         if (first && lane == 0) mbar_arrive(q_full);
-        if (!(ok = warp_wait(s_full, it & 1, abort_flag))) break;
+        if (!(ok = warp_wait(&s_full[it % L::kScores], (it / L::kScores) & 1, abort_flag))) break;
         tc_fence_after();
+        const uint32_t tS = tmem + lane_base + it % L::kScores * kKeys;
         uint32_t r[kWords][32];
 #pragma unroll
         for (int c = 0; c < kWords; ++c) tmem_ld32(tS + 32 * c, r[c]);
@@ -516,7 +523,12 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
           tmem_st16(tS + 16 * c, pk);
         }
         l = l * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
-        if (!first && __any_sync(0xffffffffu, upd)) {  // (S of this tile came after the last one's P V)
+        // O has the tile before: with one buffer this tile's S came after it
+        if (L::kScores == 2 && !first) {
+          if (!(ok = warp_wait(o_done, done++ & 1, abort_flag))) break;
+          tc_fence_after();
+        }
+        if (!first && __any_sync(0xffffffffu, upd)) {
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -684,7 +696,7 @@ int ctx_tiles_take_status(unsigned int* status) {
 
 int launch_ctx_tiles(const CtxParams& p, int D, bool fp16, int mask_tiles, bool beside, cudaStream_t s) {
   const int64_t width = 2ll * p.Hkv * D;
-  const unsigned keys = ctx_tile_keys(D);
+  const unsigned keys = kCtxTileKeys;
   CUtensorMap own{}, shared{};
   const bool use_own = p.Lkv > 0 && (p.part[0].use_own || p.part[1].use_own);
   const bool use_shared = p.part[0].use_shared != 0;
