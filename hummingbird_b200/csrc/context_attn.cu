@@ -65,7 +65,8 @@ Plan make_plan(const Shape& s) {
   p.rows_per_tile = s.D == 64 && (rows0 <= kRowsKernelMax ? rows0 : rows) > 16 ? 32 : 16;
   auto fill = [&](int i, bool pool, bool sh, bool own, int part_rows) {
     CtxPart& part = p.part[i];
-    const bool tiles = p.tiles[i] = part_rows > kRowsKernelMax;
+    const bool any = (sh && s.Ls > 0) || (own && s.Lkv > 0);  // without a key there is no tensor map to make
+    const bool tiles = p.tiles[i] = part_rows > kRowsKernelMax && any;
     part.pooled = pool;
     part.use_shared = sh;
     part.use_own = own;

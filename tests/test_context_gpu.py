@@ -122,6 +122,10 @@ def test_shared_states(cuda_lib, b, lq, lkv, ls, h, hkv, d, dtype):
 def test_no_states_gives_zeros(cuda_lib):
     q, kv, _ = _make(11, 2, 5, 4, 2, 2, 64, BF16)
     assert (_call(q, kv[:, :0], 2, 64) == 0).all()
+    for d in (64, 128):  # many rows: there is no key to make a tensor map of
+        wide, states, sh = _make(11, 2, 300, 4, 2, 2, d, BF16, ls=3)
+        assert (_call(wide, states[:, :0], 2, d) == 0).all()
+        assert (_call(wide, states[:, :0], 2, d, shared_kv=sh[:0]) == 0).all()
     assert _call(q[:, :0], kv, 2, 64).shape == (2, 0, 128)
     assert _call(q[:0], kv[:0], 2, 64).shape == (0, 5, 128)
 
