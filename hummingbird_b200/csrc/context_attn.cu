@@ -25,6 +25,7 @@ struct Plan {
   int mask_tiles;      // most key tiles of a unit of the tcgen05 kernel
   int slots, prows, tail_rows;
   size_t bytes;        // partial results
+  bool too_large;      // work units do not fit 32 bits
 };
 
 bool shape_ok(const Shape& s) {
@@ -78,6 +79,7 @@ Plan make_plan(const Shape& s) {
     // for each of the four warps) per CTA; the merge then costs less than the idle SMs.
     part.splits = std::max(1, std::min({static_cast<int>(ctas / items), chunks / (tiles ? 256 / keys : 8), kMaxSplits}));
     if (tiles && s.masked) part.splits = std::max(part.splits, ceil_div(chunks, kCtxMaskTiles));
+    if (items * part.splits >= (1ll << 30)) p.too_large = true;
     part.count = static_cast<int>(items * part.splits);
     part.slot0 = p.slots;
     p.slots += part.splits;
@@ -126,7 +128,9 @@ extern "C" int hb_context_workspace_bytes(int batch, int q_len, int kv_len, int 
   if (!bytes) return HB_ERR_NULL;
   const Shape s{batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim, masked};
   if (!shape_ok(s)) return HB_ERR_SHAPE;
-  *bytes = make_plan(s).bytes;
+  const Plan plan = make_plan(s);
+  if (plan.too_large) return HB_ERR_SHAPE;
+  *bytes = plan.bytes;
   return HB_OK;
 }
 
@@ -168,6 +172,7 @@ extern "C" int hb_context_attn(const HbContextArgs* args, cudaStream_t stream) {
       return HB_ERR_ALIGN;
   }
   const Plan plan = make_plan(s);
+  if (plan.too_large) return HB_ERR_SHAPE;
   if (plan.bytes && (!a.workspace || a.workspace_bytes < 0 || static_cast<size_t>(a.workspace_bytes) < plan.bytes))
     return HB_ERR_WORKSPACE;
   const int st = check_device();

@@ -94,6 +94,15 @@ def test_workspace_is_asked_for_and_checked(lib):
     assert lib.hb_context_workspace_bytes(1, 1, 16, 0, 16, 16, 64, 0, None) == _lib.HB_ERR_NULL
 
 
+def test_more_work_units_than_32_bits_count_are_refused(lib):
+    """A broadcast batch (stride 0) makes long masked contexts of very many elements possible: 2^22 x 1,024 units."""
+    big = dict(batch=1 << 22, q_len=40, kv_len=1 << 24, heads=1, kv_heads=1, q_bs=40 * 64, q_rs=64, kv_bs=0, kv_rs=128,
+               o_bs=40 * 64, o_rs=64, mask=P)
+    assert lib.hb_context_attn(*_args(**big)) == _lib.HB_ERR_SHAPE
+    n = ctypes.c_size_t(0)
+    assert lib.hb_context_workspace_bytes(1 << 22, 40, 1 << 24, 0, 1, 1, 64, 1, ctypes.byref(n)) == _lib.HB_ERR_SHAPE
+
+
 def test_workspace_stays_small_against_the_inputs(lib):
     """Only calls with few rows are cut along the keys, so partial results stay below a few passes over q."""
     for b, lq, lkv, ls, h, hkv, d in [(2, 2648, 8184, 0, 16, 16, 64), (8, 646, 128, 2584, 16, 16, 64),
