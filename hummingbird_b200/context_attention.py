@@ -108,7 +108,8 @@ def _attend(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_
             raise ValueError("the tensors of a context attention must be on one device")
     if device < 0:
         check_cuda(q)
-    if (q.requires_grad or kv.requires_grad or (shared_kv is not None and shared_kv.requires_grad)) \
+    if (q.requires_grad or kv.requires_grad or (shared_kv is not None and shared_kv.requires_grad)
+            or (q_weight is not None and q_weight.requires_grad) or (out is not None and out.requires_grad)) \
             and torch.is_grad_enabled():
         raise RuntimeError("context attention has no backward pass: call it under torch.no_grad()")
     q_at, kv_at = q.data_ptr(), kv.data_ptr()
@@ -150,7 +151,7 @@ def context_attention(q: torch.Tensor, kv: torch.Tensor, num_heads: int, head_di
     `lens` int32 `(B,)` and `mask` bool `(B, Lkv)` (True: read) say which states of a padded batch count; what lies
     at the others is not read, and a batch element without any gets zeros. Query head h reads kv head
     `h // (num_heads // kv_heads)`. `q_weight` `(D,)` RMS-norms every query head first (`eps`), as the DiT does.
-    `scale` defaults to `D ** -0.5`."""
+    `scale` defaults to `D ** -0.5`. `out`, where given, has 16-byte aligned rows and overlaps no input."""
     return _attend(q, None, kv, num_heads, head_dim, kv_heads, lens, mask, None, q_weight, eps, scale, out)
 
 

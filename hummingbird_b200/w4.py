@@ -111,7 +111,8 @@ def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, out_f
             or (bias is not None and bias.get_device() != device) or (out is not None and out.get_device() != device):
         check_cuda(*(t for t in (x, packed, scales, bias, out) if t is not None))
         raise ValueError("x, packed, scales, bias and out must be on one device")
-    if (x.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
+    if (x.requires_grad or scales.requires_grad or (bias is not None and bias.requires_grad)
+            or (out is not None and out.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError("W4 linear layers have no backward pass: call them under torch.no_grad()")
     x_at = x.data_ptr()
     if copy_x or x_at & 15:

@@ -242,3 +242,5 @@ def test_refuses_gradients(cuda_lib):
         _call(q, kv, 2, 64)
     with torch.no_grad():
         _check(_call(q, kv, 2, 64), q.detach(), kv, 2, 64)
+    with pytest.raises(RuntimeError):
+        _call(q.detach(), kv, 2, 64, q_weight=torch.ones(64, device="cuda", requires_grad=True))
