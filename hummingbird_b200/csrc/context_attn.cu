@@ -75,9 +75,11 @@ Plan make_plan(const Shape& s) {
     const int64_t items = (int64_t)(pool ? 1 : s.B) * s.Hkv * part.row_tiles;
     const int keys = tiles ? kCtxTileKeys : 2048 / s.D, ctas = tiles ? ctx_tile_ctas(s.D) : kCtxRowCtas;
     const int chunks = (sh ? ceil_div(s.Ls, keys) : 0) + (own ? ceil_div(s.Lkv, keys) : 0);
-    // Few items: the key list is cut so that one round of CTAs fills the GPU, down to 256 keys (or two chunks
-    // for each of the four warps) per CTA; the merge then costs less than the idle SMs.
+    // Few items: the key list is cut so that one round of CTAs fills the GPU, down to 256 keys (or two chunks for each
+    // of the four warps) per CTA. Below 24 chunks the few-rows kernel walks the list whole in the time that the merge
+    // takes (17 tokens of 234 keys at D 128: 6.3 us whole, 7.5 cut; one token of 1,000 keys: 8.0 whole, 5.8 cut).
     part.splits = std::max(1, std::min({static_cast<int>(ctas / items), chunks / (tiles ? 256 / keys : 8), kMaxSplits}));
+    if (!tiles && chunks < 24) part.splits = 1;
     if (tiles && s.masked) part.splits = std::max(part.splits, ceil_div(chunks, kCtxMaskTiles));
     if (items * part.splits >= (1ll << 30)) p.too_large = true;
     part.count = static_cast<int>(items * part.splits);
