@@ -119,6 +119,57 @@ def test_shared_states(cuda_lib, b, lq, lkv, ls, h, hkv, d, dtype):
     assert (empty == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("b,lq,lkv,ls,h,hkv,d", [
+    (2, 1, 7, 70000, 8, 2, 64),      # pooled rows and own rows in the few-rows kernel
+    (33, 1, 257, 4200, 8, 2, 64),    # pooled rows in the tcgen05 kernel, own rows beside it
+    (6, 60, 33, 16000, 4, 2, 64),    # both in the tcgen05 kernel
+    (24, 3, 65, 3100, 6, 2, 128),
+])
+def test_long_shared_states_are_pooled(cuda_lib, b, lq, lkv, ls, h, hkv, d, dtype):
+    """Long enough shared states that all batch elements' rows take them in one pass, apart from their own."""
+    assert (b - 1) * ls * hkv * d * 4 > 32 << 20 and lq * h // hkv < 128
+    q, kv, sh = _make(30, b, lq, lkv, h, hkv, d, dtype, ls=ls)
+    g = torch.Generator().manual_seed(31)
+    lens = torch.randint(0, lkv + 1, (b,), generator=g, dtype=torch.int32).cuda()
+    lens[0] = 0
+    valid = torch.arange(lkv, device="cuda")[None] < lens[:, None]
+    kw = dict(kv_heads=hkv, lens=lens)
+    out = _call(q, kv.masked_fill(~valid[..., None], float("nan")), h, d, shared_kv=sh, **kw)
+    _check(out, q, kv, h, d, shared_kv=sh, **kw)
+    smask = (torch.rand(ls, generator=g) < 0.5).cuda()
+    smask[100:1000] = False
+    kw["shared_mask"] = smask
+    dirty = sh.masked_fill(~smask[:, None], float("inf"))
+    _check(_call(q, kv, h, d, shared_kv=dirty, **kw), q, kv, h, d, shared_kv=sh, **kw)
+    none = kv[:, :0]
+    _check(_call(q, none, h, d, shared_kv=sh, kv_heads=hkv), q, none, h, d, shared_kv=sh, kv_heads=hkv)
+
+
+@pytest.mark.parametrize("lq,lkv,ls,h,hkv,d", [(10200, 1000, 0, 8, 4, 64), (4700, 900, 300, 16, 16, 64),
+                                               (9590, 1100, 0, 4, 4, 128)])
+def test_items_of_a_last_round_are_cut(cuda_lib, lq, lkv, ls, h, hkv, d):
+    """More tiles of rows than run at once: the last round's key lists are cut and merged; rows sampled from every
+    tile, the last, partly empty one whole."""
+    q, kv, sh = _make(32, 1, lq, lkv, h, hkv, d, BF16, ls=ls)
+    out = _call(q, kv, h, d, kv_heads=hkv, shared_kv=sh)
+    rows = torch.cat([torch.arange(0, lq, 61), torch.arange(lq - 130, lq)]).unique().cuda()
+    _check(out[:, rows], q[:, rows], kv, h, d, kv_heads=hkv, shared_kv=sh)
+    assert torch.isfinite(out).all()
+
+
+def test_long_masked_context_of_many_rows(cuda_lib):
+    """Mask bits of more keys than a CTA holds: the key list is cut however many rows there are."""
+    lq, lkv = 76000, 17000
+    q, kv, _ = _make(33, 1, lq, lkv, 1, 1, 64, FP16)
+    mask = (torch.rand(1, lkv, generator=torch.Generator().manual_seed(34)) < 0.5).cuda()
+    mask[0, 3000:9000] = False
+    out = _call(q, kv.masked_fill(~mask[..., None], float("nan")), 1, 64, mask=mask)
+    rows = torch.arange(0, lq, 997).cuda()
+    _check(out[:, rows], q[:, rows], kv, 1, 64, mask=mask)
+    assert torch.isfinite(out).all()
+
+
 def test_no_states_gives_zeros(cuda_lib):
     q, kv, _ = _make(11, 2, 5, 4, 2, 2, 64, BF16)
     assert (_call(q, kv[:, :0], 2, 64) == 0).all()
@@ -194,7 +245,7 @@ def test_large_scores(cuda_lib):
 
 
 def test_same_call_same_bits_and_streams(cuda_lib):
-    q, kv, sh = _make(18, 4, 2, 3000, 8, 2, 64, BF16, ls=5000)
+    q, kv, sh = _make(18, 4, 2, 3000, 8, 2, 64, BF16, ls=22000)  # pooled: two kernels and a merge
     ref = _call(q, kv, 8, 64, shared_kv=sh, kv_heads=2)
     for _ in range(3):
         assert torch.equal(_call(q, kv, 8, 64, shared_kv=sh, kv_heads=2), ref)
@@ -212,7 +263,7 @@ def test_same_call_same_bits_and_streams(cuda_lib):
 
 def test_two_graphs_replayed_together(cuda_lib):
     """Two captured calls with split key lists, replayed on two streams at once, each on inputs refilled in place."""
-    sets = [_make(20 + i, 2, 1, 6000, 8, 2, 64, BF16, ls=4000) for i in range(2)]
+    sets = [_make(20, 2, 1, 6000, 8, 2, 64, BF16, ls=70000), _make(21, 9, 4, 2000, 8, 2, 64, BF16, ls=9000)]
     graphs, outs = [], []
     for q, kv, sh in sets:
         _call(q, kv, 8, 64, shared_kv=sh, kv_heads=2)
