@@ -20,16 +20,20 @@ def check_cuda(*tensors: torch.Tensor) -> None:
             raise RuntimeError("hummingbird_b200 operators run on CUDA tensors only (there is no CPU path)")
 
 
-try:  # the current stream's handle without building a torch.cuda.Stream around it (2 us)
+try:  # the current stream's handle and device without the torch.cuda wrappers around them (2 us)
     from torch._C import _cuda_getCurrentRawStream as raw_stream
+    from torch._C import _cuda_getDevice as current_device
 except ImportError:
+    current_device = torch.cuda.current_device
+
     def raw_stream(device: int) -> int:
         return torch.cuda.current_stream(device).cuda_stream
 
 
 def launch(device: int, name: str, fn, args) -> None:
-    """Call entry point `fn(args, stream)` on the current stream of CUDA device `device`, with that device current."""
-    if torch.cuda.current_device() == device:
+    """Call entry point `fn(args, stream)` on the current stream of CUDA device `device`, with that device current
+    (a tensor lives there, so CUDA is initialised)."""
+    if current_device() == device:
         code = fn(args, raw_stream(device))
     else:
         with torch.cuda.device(device):

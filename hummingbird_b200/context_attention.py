@@ -26,8 +26,8 @@ _PLANS: dict = {}                   # checked calls by the sizes, strides and ty
 _MAX_PLANS = 4096
 
 
-def _layout(t: torch.Tensor | None):
-    return None if t is None else (t.shape, t.stride(), t.dtype)
+def _layout(t: torch.Tensor):
+    return t.shape, t.stride(), t.dtype
 
 
 def _readable(t: torch.Tensor, width: int) -> bool:
@@ -82,7 +82,8 @@ def _plan(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_ma
     strides = (q.stride(0), q.stride(1), kv.stride(0), kv.stride(1), 0 if shared_kv is None else shared_kv.stride(0),
                0 if mask is None else mask.stride(0))
     sizes = (batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim, _DTYPES[dtype])
-    return any(copies) and copies, need, strides, sizes, q.is_contiguous() and batch * q_len > 0
+    return (any(copies) and copies, need, strides, sizes, q.is_contiguous() and batch * q_len > 0,
+            _lib.lib().hb_context_attn)
 
 
 def _own_copy(t: torch.Tensor, copy: bool, dtype=None):
@@ -93,21 +94,24 @@ def _attend(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_
     if kv_heads is None:
         kv_heads = num_heads
     key = (num_heads, head_dim, kv_heads, q.shape, q.stride(), q.dtype, kv.shape, kv.stride(), kv.dtype,
-           _layout(shared_kv), _layout(lens), _layout(mask), _layout(shared_mask), _layout(q_weight), _layout(out))
+           None if shared_kv is None else _layout(shared_kv), None if lens is None else _layout(lens),
+           None if mask is None else _layout(mask), None if shared_mask is None else _layout(shared_mask),
+           None if q_weight is None else _layout(q_weight), None if out is None else _layout(out))
     plan = _PLANS.get(key)
     if plan is None:
         plan = _plan(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_mask, q_weight, out)
         if len(_PLANS) >= _MAX_PLANS:
             _PLANS.clear()
         _PLANS[key] = plan
-    copies, need, strides, sizes, like_q = plan
+    copies, need, strides, sizes, like_q, call = plan
     device = q.get_device()
-    for t in (kv, shared_kv, lens, mask, shared_mask, q_weight, out):
-        if t is not None and t.get_device() != device:
-            check_cuda(q, t)
-            raise ValueError("the tensors of a context attention must be on one device")
-    if device < 0:
-        check_cuda(q)
+    if device < 0 or kv.get_device() != device or (shared_kv is not None and shared_kv.get_device() != device) \
+            or (lens is not None and lens.get_device() != device) or (mask is not None and mask.get_device() != device) \
+            or (shared_mask is not None and shared_mask.get_device() != device) \
+            or (q_weight is not None and q_weight.get_device() != device) \
+            or (out is not None and out.get_device() != device):
+        check_cuda(*(t for t in (q, kv, shared_kv, lens, mask, shared_mask, q_weight, out) if t is not None))
+        raise ValueError("the tensors of a context attention must be on one device")
     if (q.requires_grad or kv.requires_grad or (shared_kv is not None and shared_kv.requires_grad)
             or (q_weight is not None and q_weight.requires_grad) or (out is not None and out.requires_grad)) \
             and torch.is_grad_enabled():
@@ -132,13 +136,13 @@ def _attend(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_
         return out
     # Partial results in a block of the caching allocator: it belongs to this call's stream, or to the graph that is
     # being captured, so calls on other streams and other graphs have theirs.
-    ws = q.new_empty(need, dtype=torch.uint8) if need else None
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     out_strides = out.stride()
     args = _ARGS.pack(q_at, kv_at, shared_at, 0 if lens is None else lens.data_ptr(),
                       0 if mask is None else mask.data_ptr(), 0 if shared_mask is None else shared_mask.data_ptr(),
                       weight_at, out.data_ptr(), 0 if ws is None else ws.data_ptr(), *strides, out_strides[0],
                       out_strides[1], need, *sizes, eps, head_dim ** -0.5 if scale is None else scale)
-    launch(device, "hb_context_attn", _lib.lib().hb_context_attn, args)
+    launch(device, "hb_context_attn", call, args)
     return out
 
 

@@ -122,7 +122,7 @@ def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, out_f
         bias = bias.contiguous()
     m, k = x.shape
     if out is None:
-        out = x.new_empty((m, out_features))
+        out = torch.empty(m, out_features, dtype=x.dtype, device=x.device)
     if m:
         launch(device, "hb_w4_linear", _lib.lib().hb_w4_linear,
                _ARGS.pack(x_at, packed.data_ptr(), scales.data_ptr(), 0 if bias is None else bias.data_ptr(),
