@@ -21,7 +21,7 @@
 // are zeroed in shared memory (0 * NaN would reach O); tiles without any valid key are skipped by every role.
 //
 // Batch 2, 2,648 queries, 16 heads, 8,184 keys, D 64: 234 us, 760 TFLOP/s, 46 % of the measured bf16 rate; issue slots
-// 61 % used, MUFU 55 %, tensor pipe 36 %. At D 128 about 345 us, 1,030 TFLOP/s, 63 %.
+// 61 % used, MUFU 55 %, tensor pipe 36 %. At D 128 326 us, 1,090 TFLOP/s, 66 %.
 //
 // Compiled as whole-program device code, as setmaxnreg needs; its status word is read by hb_device_status.
 #define HB_WHOLE_PROGRAM 1
