@@ -114,7 +114,7 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 
 // NT: groups of eight rows of x. RT: tiles of 16 outputs that share what a warp reads of x.
 template <bool kFp16, int NT, int RT, int kGroup>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 8 : NT == 2 ? 4 : 3 - RT / 2) w4_linear_kernel(const W4Params p) {
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 6 : NT == 2 ? 4 : 3 - RT / 2) w4_linear_kernel(const W4Params p) {
   using T = Half<kFp16>;
   constexpr int kSteps = kGroup / 32;        // word steps per group
   constexpr int kGroups = 128 / kGroup;      // groups per block
