@@ -199,7 +199,7 @@ __device__ __forceinline__ void st_32b(void* dst, const uint32_t* v) {
 template <int D, bool kFp16, bool kMask>
 __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
     ctx_tiles_kernel(const __grid_constant__ CUtensorMap tm_own, const __grid_constant__ CUtensorMap tm_shared,
-                     const __grid_constant__ CtxParams p, const int mask_tiles) {
+                     const __grid_constant__ CtxParams p, const int mask_tiles, const int beside) {
   using L = Layout<D>;
   constexpr int kStages = L::kStages, kKeys = L::kKeys, kWords = L::kWords;
   constexpr int PPR = D / 8;  // 16-byte pieces per row
@@ -222,7 +222,6 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
   uint32_t* bits0 = reinterpret_cast<uint32_t*>(smem + L::kOffBits);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge, which waits for this kernel
   const int count0 = p.part[0].count, total = count0 + p.part[1].count;
 
   if (warp == 4 && lane == 0) {
@@ -275,6 +274,11 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // Up to here nothing but parameters was read, so this may run while the kernel before still does (a call among others
+  // 20.5 -> 19.1 us at the 120 s clip's cross-attention). The launch beside the few-rows kernel does not wait for that
+  // one here: it was let in by a kernel that had waited itself.
+  if (!beside) asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge, or the next early launch: they wait
   if (warp < 4) load_q(blockIdx.x);
   tc_fence_before();
   __syncthreads();
@@ -677,7 +681,8 @@ int launch_tiles(const CUtensorMap& own, const CUtensorMap& shared, const CtxPar
     if (dev < 64) configured[dev] = true;
   }
   const int grid = std::min(p.part[0].count + p.part[1].count, ctx_tile_ctas(D));
-  return launch_after(beside, kernel, grid, kThreads, Layout<D>::bytes(mask_tiles), s, own, shared, p, mask_tiles);
+  return launch_after(true, kernel, grid, kThreads, Layout<D>::bytes(mask_tiles), s, own, shared, p, mask_tiles,
+                      static_cast<int>(beside));
 }
 
 template <int D, bool kFp16>
