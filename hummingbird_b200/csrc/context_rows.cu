@@ -427,13 +427,13 @@ int launch_rows(const CtxParams& p, cudaStream_t s) {
       return HB_ERR_LAUNCH;
     if (dev < 64) configured[dev] = true;
   }
-  return launch_after(false, ctx_rows_kernel<D, T, MT>, p.part[0].count + p.part[1].count, 32 * kWarps, kRowsSmem, s, p);
+  return launch_after(ctx_rows_kernel<D, T, MT>, p.part[0].count + p.part[1].count, 32 * kWarps, kRowsSmem, s, p);
 }
 
 template <int D, class T, int kTeams>
 int launch_teams(const CtxParams& p, cudaStream_t s) {
   const int64_t threads = (int64_t)p.prows * (D / 4) * kTeams;
-  return launch_after(true, ctx_combine_kernel<D, T, kTeams>, static_cast<unsigned>((threads + 255) / 256), 256, 0, s, p);
+  return launch_after(ctx_combine_kernel<D, T, kTeams>, static_cast<unsigned>((threads + 255) / 256), 256, 0, s, p);
 }
 // As many teams as it takes to have about a thousand threads on every SM, and no more than have slots to read.
 template <int D, class T>

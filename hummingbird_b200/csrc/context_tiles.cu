@@ -681,7 +681,7 @@ int launch_tiles(const CUtensorMap& own, const CUtensorMap& shared, const CtxPar
     if (dev < 64) configured[dev] = true;
   }
   const int grid = std::min(p.part[0].count + p.part[1].count, ctx_tile_ctas(D));
-  return launch_after(true, kernel, grid, kThreads, Layout<D>::bytes(mask_tiles), s, own, shared, p, mask_tiles,
+  return launch_after(kernel, grid, kThreads, Layout<D>::bytes(mask_tiles), s, own, shared, p, mask_tiles,
                       static_cast<int>(beside));
 }
 

@@ -6,13 +6,13 @@
 
 namespace hb {
 
-// Launch a kernel that, where `early`, may begin once every CTA of the one before it has started and allowed it
+// Launch a kernel that may begin once every CTA of the one before it has started and allowed it
 // (griddepcontrol.launch_dependents), or else when that one is done: its setup then costs no time of its own. A kernel
 // launched so reads and writes nothing but its parameters before griddepcontrol.wait, which returns when the one
 // before is complete with its memory visible, and allows the next one only after that; or it reads nothing that the
 // one before writes, was let in by a kernel that had waited itself, and waits before it ends.
 template <class... P, class... A>
-int launch_after(bool early, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+int launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
                  const A&... args) {
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -23,7 +23,7 @@ int launch_after(bool early, void (*kernel)(P...), dim3 grid, unsigned threads, 
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = &attr;
-  cfg.numAttrs = early ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? HB_OK : HB_ERR_LAUNCH;
 }
 

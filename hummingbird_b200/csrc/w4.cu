@@ -15,7 +15,7 @@
 // One CTA takes 16 outputs (or 32); its four warps take every fourth block of 128 inputs, each through a ring of
 // asynchronous copies of its own, and merge through shared memory in warp order, so the result does not depend on
 // timing. x is read through L1 (it is the same few rows for every CTA).
-// One row, 16,384 x 8,192, group 128: 17.8 us, 3.9 TB/s, 59 % of the measured copy rate; unpacking bounds it (the
+// One row, 16,384 x 8,192, group 128: 17.6 us, 3.9 TB/s, 60 % of the measured copy rate; unpacking bounds it (the
 // integer pipe is busy half of the time, instruction issue 60 %; 22 us with two logic operations to a nibble pair).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -295,12 +295,10 @@ __global__ void __launch_bounds__(256) w4_quant_kernel(const uint16_t* __restric
 
 template <bool kFp16, int NT, int RT>
 int launch_linear(const W4Params& p, int group, cudaStream_t s) {
-  // (an early start: 1,024 x 256 1.8 -> 1.6 us, 6,144 x 1,024 3.0 -> 2.8; 16,384 x 8,192 17.8 -> 19.2)
-  const bool early = (int64_t)p.N * p.K <= 16 << 20;
   const dim3 grid((p.N + 16 * RT - 1) / (16 * RT), (p.M + 8 * NT - 1) / (8 * NT));
-  if (group == 32) return launch_after(early, w4_linear_kernel<kFp16, NT, RT, 32>, grid, 32 * kWarps, 0, s, p);
-  if (group == 64) return launch_after(early, w4_linear_kernel<kFp16, NT, RT, 64>, grid, 32 * kWarps, 0, s, p);
-  return launch_after(early, w4_linear_kernel<kFp16, NT, RT, 128>, grid, 32 * kWarps, 0, s, p);
+  if (group == 32) return launch_after(w4_linear_kernel<kFp16, NT, RT, 32>, grid, 32 * kWarps, 0, s, p);
+  if (group == 64) return launch_after(w4_linear_kernel<kFp16, NT, RT, 64>, grid, 32 * kWarps, 0, s, p);
+  return launch_after(w4_linear_kernel<kFp16, NT, RT, 128>, grid, 32 * kWarps, 0, s, p);
 }
 template <bool kFp16>
 int launch_linear(const W4Params& p, int group, cudaStream_t s) {
