@@ -390,7 +390,10 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
           j = jn;
           n16 = n16_next;
         }
-        if (kMask && lead) mbar_arrive(&m_free[n & 1]);
+        if constexpr (kMask) {
+          __syncwarp();  // every lane has read the unit's mask bits
+          if (lead) mbar_arrive(&m_free[n & 1]);
+        }
       }
       commit(lead, drain);  // every MMA this thread issued has finished before TMEM is freed
       mbar_wait(drain, 0);
@@ -575,7 +578,10 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
         ++it;
         first = false;
       }
-      if (kMask && lane == 0) mbar_arrive(&m_free[n & 1]);
+      if constexpr (kMask) {
+        __syncwarp();  // every lane has read the unit's mask bits
+        if (lane == 0) mbar_arrive(&m_free[n & 1]);
+      }
       // -------------------------------------------------------------- epilogue: one row per thread
       if (!ok) break;
       if (w + gridDim.x < total) load_q(w + gridDim.x);  // (the S MMAs of this unit are done)

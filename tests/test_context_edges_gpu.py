@@ -1,0 +1,61 @@
+"""GPU: context attention at its edges: mask buffers handed from unit to unit, launches that overlap, values that are
+not finite, weights far below the largest one, key lists that are cut for a last round of CTAs."""
+import numpy as np
+import pytest
+import torch
+
+from oracle.context import context_attention as plain
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+UNIT = {BF16: 2.0 ** -8, FP16: 2.0 ** -11}
+
+
+def _np(t):
+    return None if t is None else t.double().cpu().numpy() if t.is_floating_point() else t.cpu().numpy()
+
+
+def _make(seed, b, lq, lkv, h, hkv, d, dtype, ls=0):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(b, lq, h * d, generator=g).to(dtype).cuda()
+    kv = torch.randn(b, lkv, 2 * hkv * d, generator=g).to(dtype).cuda()
+    sh = torch.randn(ls, 2 * hkv * d, generator=g).to(dtype).cuda() if ls else None
+    return q, kv, sh
+
+
+def _call(q, kv, h, d, shared_kv=None, **kw):
+    from hummingbird_b200.context_attention import context_attention, shared_context_attention
+    if shared_kv is None:
+        return context_attention(q, kv, h, d, **kw)
+    return shared_context_attention(q, shared_kv, kv, h, d, **kw)
+
+
+def _check(out, q, kv, h, d, **kw):
+    ref, tol = plain(_np(q), np.nan_to_num(_np(kv), posinf=0, neginf=0), h, d, unit=UNIT[q.dtype],
+                     **{k: _np(v) if torch.is_tensor(v) else v for k, v in kw.items()})
+    got = _np(out)
+    assert np.isfinite(got).all(), "non-finite output"
+    over = np.abs(got - ref) - tol
+    assert over.max() <= 0, f"off by {np.abs(got - ref).max():.3e}, {over.max():.3e} over the bound"
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("b,lq,h,d", [(3, 2000, 16, 64), (3, 2000, 8, 128)])
+def test_units_without_keys_between_masked_ones(cuda_lib, b, lq, h, d, dtype):
+    """Several units to a CTA (768 on 592, 384 on 296), so its two mask buffers are filled again and again: one batch
+    element whose last tiles hold no valid key (every role skips them and gives the buffer back), one without any key,
+    one with a single key in the last tile."""
+    lkv = 401
+    q, kv, _ = _make(40, b, lq, lkv, h, h, d, dtype)
+    mask = (torch.rand(b, lkv, generator=torch.Generator().manual_seed(41)) < 0.5).cuda()
+    mask[0, 0], mask[0, 70:] = True, False
+    mask[1] = False
+    mask[2, 64:], mask[2, 400] = False, True
+    dirty = kv.masked_fill(~mask[..., None], float("nan"))
+    ref = _call(q, dirty, h, d, mask=mask)
+    assert (ref[1] == 0).all() and torch.isfinite(ref).all()
+    rows = torch.arange(0, lq, 53).cuda()
+    _check(ref[:, rows], q[:, rows], dirty, h, d, mask=mask)
+    for _ in range(5):
+        assert torch.equal(_call(q, dirty, h, d, mask=mask), ref)
