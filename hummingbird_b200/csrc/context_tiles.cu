@@ -278,12 +278,14 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
   // 20.5 -> 19.1 us at the 120 s clip's cross-attention). The launch beside the few-rows kernel does not wait for that
   // one here: it was let in by a kernel that had waited itself.
   if (!beside) asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge, or the next early launch: they wait
   if (warp < 4) load_q(blockIdx.x);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // The merge, or the next early launch: they wait. Not before every CTA of this launch has its TMEM: a CTA of the next
+  // one keeps its columns while it waits for this launch, and must not hold what this one still asks for.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp >= 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kOtherRegs));

@@ -59,3 +59,25 @@ def test_units_without_keys_between_masked_ones(cuda_lib, b, lq, h, d, dtype):
     _check(ref[:, rows], q[:, rows], dirty, h, d, mask=mask)
     for _ in range(5):
         assert torch.equal(_call(q, dirty, h, d, mask=mask), ref)
+
+
+def test_early_launches_of_both_head_dims_on_two_streams(cuda_lib):
+    """Each launch may start under the end of the one before it, and its CTAs then hold tensor memory while they wait:
+    calls that take 128 and 256 columns a CTA in turn, on two streams at once, more CTAs than run at once."""
+    sets = [(*_make(42 + i, b, lq, 300, h, h, d, BF16)[:2], h, d)
+            for i, (b, lq, h, d) in enumerate([(2, 700, 16, 64), (1, 900, 6, 128), (1, 130, 2, 64), (2, 1500, 16, 128)])]
+    refs = [_call(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    outs = []
+    for turn in range(12):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                for i in range(len(sets)):
+                    j = (i * (k + 1) + turn) % len(sets)
+                    outs.append((j, _call(*sets[j])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, refs[j]) for j, out in outs)
+    from hummingbird_b200 import _lib
+    assert _lib.device_status() == 0
