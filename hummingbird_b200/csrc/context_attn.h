@@ -68,7 +68,7 @@ struct CtxParams {
   // the last items of part[1] are cut (`tail_rows` > 0 rows per tile), for the rows of those items' tiles.
   int slots, prows, tail_rows;
   float* o_part;          // [slots][prows][D]: sum of p * v
-  float2* ml_part;        // [slots][prows]: running maximum (log2 units; -inf: no key), sum of p
+  float2* ml_part;        // [slots][prows]: the exponent that p is relative to (log2; -inf: no key), sum of p
 };
 
 // A work unit: tile `rt` of the rows of kv head g (batch element b; all of them where pooled), keys

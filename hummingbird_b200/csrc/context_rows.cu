@@ -30,7 +30,11 @@ constexpr int kChunkBytes = 8192;  // K and V of one chunk
 constexpr int kWarpBytes = kStages * kChunkBytes;
 constexpr int kRowsSmem = kWarps * kWarpBytes + kWarps * kStages * 4 + kWarps * 32 * 8;
 
+// kLift: all weights p <= 1 are multiplied by 2^kLift, so that small ones stay in the type's normal range for P V. fp16's
+// ends at 2^-14 (its subnormals at 2^-24): lifted, weights down to 2^-29 of the largest keep 11 bits, smaller ones are off
+// by at most 2^-40 of it.
 struct Bf16 {
+  static constexpr float kLift = 0.f;
   static __device__ __forceinline__ float2 unpack(uint32_t w) { return {bf16_lo(w), bf16_hi(w)}; }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
   static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -41,6 +45,7 @@ struct Bf16 {
   }
 };
 struct Fp16 {
+  static constexpr float kLift = 15.f;
   static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     __half2 h = __floats2half2_rn(a, b);
@@ -245,7 +250,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
           const float mn = fmaxf(m[mt][hf], mx[hf] * p.scale_log2);
           const float alpha = mn == -INFINITY ? 1.f : ex2_approx(m[mt][hf] - mn);
           m[mt][hf] = mn;
-          nm[hf] = mn == -INFINITY ? 0.f : -mn;
+          nm[hf] = mn == -INFINITY ? 0.f : T::kLift - mn;
           l[mt][hf] *= alpha;
 #pragma unroll
           for (int i = 0; i < D / 8; ++i) {
@@ -261,7 +266,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
             e[j] = ex2_approx(fmaf(s[mt][i][j], p.scale_log2, nm[j >> 1]));
             l[mt][j >> 1] += e[j];
           }
-          // P in the input's type for the MMA (at most 1, relative error up to 2^-8 or 2^-11); l keeps fp32
+          // P in the input's type for the MMA (relative error up to 2^-8 or 2^-11); l keeps fp32
           pf[mt][i >> 1][(i & 1) * 2] = T::pack(e[0], e[1]);
           pf[mt][i >> 1][(i & 1) * 2 + 1] = T::pack(e[2], e[3]);
         }
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
       *reinterpret_cast<uint4*>(p.out + x.bq * p.o_bs + x.i * p.o_rs + (int64_t)x.hq * D + ch * 8) = w;
     } else {
       const int64_t pr = ctx_prow(p, part, u, x, row);
-      if (ch == 0) p.ml_part[pr] = make_float2(mx, sum);
+      if (ch == 0) p.ml_part[pr] = make_float2(mx - T::kLift, sum);
       float4* dst = reinterpret_cast<float4*>(p.o_part + pr * D + ch * 8);
       dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
       dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);

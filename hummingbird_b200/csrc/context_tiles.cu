@@ -8,7 +8,7 @@
 // scores 660 to 800 at D 64; and within a tile S, softmax and P V wait for one another, about as long again. So at D 64
 // four CTAs share an SM, as many as TMEM holds their S and O for (64 + 64 columns), and fill each other's waits. At
 // D 128 there is room for two, each with two buffers of S (2 x 64 + 128 columns): the next tile's S runs while this
-// one's softmax does. A lazy maximum (O is rescaled only when a row's maximum grows by more than 2^8) keeps O in
+// one's softmax does. A lazy maximum (O is rescaled only when a row's maximum grows by more than 2^8, in fp16 2^4) keeps O in
 // TMEM, and a share of the exponentials goes to the FMA pipe (exp2_poly2).
 //
 // The grid is one round of CTAs; each walks its share of the units (tiles of rows), so barriers, TMEM and tensor maps
@@ -41,7 +41,15 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kQAtom = 128 * 128;                // 128 rows of 128 bytes: 64 columns of a query tile
-constexpr float kRescaleThreshold = 8.0f;        // log2 units
+// By how much (log2 units) a row's maximum may grow before O is rescaled, and what all weights are multiplied by (2^kLift)
+// so that small ones stay in P's normal range; P is at most 2^(kRescaleThreshold + kLift). bf16 has fp32's range. fp16's
+// normal range ends at 2^-14, its subnormal at 2^-24: lifted, weights down to 2^-25 of the largest keep 11 bits and
+// smaller ones are off by at most 2^-36 of it, 2^-11 in all over 2^25 keys (unlifted, 131,072 keys of weight 2^-25.2 beside
+// one of 1 were lost whole).
+template <bool kFp16>
+constexpr float kRescaleThreshold = kFp16 ? 4.f : 8.f;
+template <bool kFp16>
+constexpr float kLift = kFp16 ? 11.f : 0.f;
 constexpr int kCtxPolyMask = 3;                  // key pairs j with (j & 3) == 3 take exp2_poly2
 
 template <int D>
@@ -505,13 +513,13 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
             mx[e / 2 & 3] = fmax3(mx[e / 2 & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
         const float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
         const float m_new = fmaxf(m, rmax);
-        const bool upd = m_new > m + kRescaleThreshold;
+        const bool upd = m_new > m + kRescaleThreshold<kFp16>;
         float alpha = 1.f;
         if (upd) {
           alpha = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
           m = m_new;
         }
-        const float nm = m == -INFINITY ? 0.f : -m;
+        const float nm = m == -INFINITY ? 0.f : kLift<kFp16> - m;
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < kWords; ++c) {
@@ -529,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
             }
             const int a2 = (e & 1) * 2;
             fadd2(rs[a2], rs[a2 + 1], rs[a2], rs[a2 + 1], p0, p1);
-            // P in the input's type for the MMA (at most 2^8 above 1, relative error up to 2^-8 or 2^-11)
+            // P in the input's type for the MMA (relative error up to 2^-8 or 2^-11); l keeps fp32
             pk[e] = pack16<kFp16>(p0, p1);
           }
           tmem_st16(tS + 16 * c, pk);
@@ -618,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
         }
       } else {
         const int64_t pr = ctx_prow(p, part, u, x, row);
-        if (live) p.ml_part[pr] = make_float2(l == 0.f ? -INFINITY : m, l);
+        if (live) p.ml_part[pr] = make_float2(l == 0.f ? -INFINITY : m - kLift<kFp16>, l);
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];

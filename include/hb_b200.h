@@ -148,7 +148,8 @@ typedef struct HbContextArgs {
  *   dtype     HB_BF16 or HB_FP16, for q, kv, shared_kv and out alike.
  * A row without a valid key is written as zeros; what lies at keys that are not valid (infinities, NaN) does not
  * reach the result. Scores, softmax statistics and sums are fp32; the weights p are rounded to the 16-bit type for
- * the product with v (relative error at most 2^-8 or 2^-11 each), the sum of p is not. head_dim 64 or 128; rows of q,
+ * the product with v (relative error at most 2^-8 or 2^-11 each; in fp16 a weight below 2^-25 of the row's largest may
+ * be off by 2^-36 of that instead), the sum of p is not; exponentials are good to 7.5e-5. head_dim 64 or 128; rows of q,
  * kv, shared_kv, out and their strides 16-byte aligned, workspace 32-byte; kv's batch stride 0, or one of its two
  * strides a multiple of the other; kv_len and shared_len at most 2^24; scale > 0. The result does not depend on
  * timing: the same call gives the same bits. Calls that may overlap on the GPU need workspaces of their own. */

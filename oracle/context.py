@@ -12,8 +12,9 @@ EXP2_ERROR = 8e-5  # of the polynomial that takes a share of the exponentials (i
 
 
 def context_attention(q, kv, heads, head_dim, *, kv_heads=None, lens=None, mask=None, shared_kv=None,
-                      shared_mask=None, q_weight=None, eps=1e-6, scale=None, unit=2.0 ** -8):
-    """`(out, tol)`, both `(B, Lq, H * D)` float64. `unit` is the 16-bit type's largest relative rounding error.
+                      shared_mask=None, q_weight=None, eps=1e-6, scale=None, unit=2.0 ** -8, floor=0.0):
+    """`(out, tol)`, both `(B, Lq, H * D)` float64. `unit` is the 16-bit type's largest relative rounding error, `floor`
+    what a weight below the type's normal range may be off by, in units of the row's largest weight.
 
     tol, element by element, with A = sum_j p_j |v_j|: the output's own rounding (unit |o|), the weights' rounding
     (unit A), scores off by delta (fp32 sums of D products, the normed query's rounding where there is a norm, the
@@ -55,4 +56,5 @@ def context_attention(q, kv, heads, head_dim, *, kv_heads=None, lens=None, mask=
             o, a = p @ v, p @ np.abs(v)
             out[b, :, cols] = o
             tol[b, :, cols] = unit * (a + np.abs(o)) * (1 + unit) + np.expm1(2 * delta) * a + n * 2.0 ** -23 * a
+            tol[b, :, cols] += floor * p.max(-1, keepdims=True) * np.abs(v).sum(0)
     return out, tol

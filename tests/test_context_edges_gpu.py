@@ -81,3 +81,30 @@ def test_early_launches_of_both_head_dims_on_two_streams(cuda_lib):
     assert all(torch.equal(out, refs[j]) for j, out in outs)
     from hummingbird_b200 import _lib
     assert _lib.device_status() == 0
+
+
+FP16_FLOOR = 2.0 ** -36  # of the row's largest weight: the error of an fp16 weight below the type's normal range
+
+
+@pytest.mark.parametrize("gap", [14.3, 17.0, 21.3, 25.2, 29.0])
+@pytest.mark.parametrize("b,lq,d", [(300, 1, 64), (600, 40, 64), (300, 40, 128), (1, 1, 64), (1, 200, 128)])
+def test_fp16_weights_far_below_the_largest(cuda_lib, b, lq, d, gap):
+    """One key with weight 1 and value 0 in front of 20,000 whose weights are 2^-gap and whose values are 1: fp16's
+    normal range ends at 2^-14, and what is lost below it adds up. Key lists walked whole by either kernel (many batch
+    elements) and cut."""
+    n = 20000
+    kv = torch.zeros(1, n + 1, 2 * d, dtype=FP16)
+    kv[0, 0, :d] = gap * np.log(2) / d ** 0.5
+    kv[0, 1:, :d] = 0.01 * torch.randn(n, d, generator=torch.Generator().manual_seed(50))
+    kv[0, 1:, d:] = 1.0
+    kv = kv.cuda().expand(b, -1, -1)
+    q = torch.ones(b, lq, d, dtype=FP16, device="cuda")
+    q[:, 1::2] = 0.75
+    out = _call(q, kv, 1, d)
+    pick = torch.tensor(sorted({0, b // 2, b - 1}))
+    rows = torch.arange(min(2, lq))
+    ref, tol = plain(_np(q[pick][:, rows]), _np(kv[pick]), 1, d, unit=UNIT[FP16], floor=FP16_FLOOR)
+    got = _np(out[pick][:, rows])
+    over = np.abs(got - ref) - tol
+    assert over.max() <= 0, f"{got.flat[0]:.4e} instead of {ref.flat[0]:.4e}, bound {tol.flat[0]:.1e}"
+    assert torch.equal(out[0, :lq], out[b - 1, :lq])
