@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(256) ctx_combine_kernel(const CtxParams p) {
 #pragma unroll 4
     for (int s = team; s < p.slots; s += kTeams) {
       const float2 ml = p.ml_part[(int64_t)s * p.prows + row];
-      if (ml.x == -INFINITY) continue;  // a part without keys left its sums unwritten
+      if (ml.y == 0.f) continue;  // a part without keys left its sums unwritten (a NaN row's maximum is -inf too, its sum NaN)
       const float f = ex2_approx(ml.x - mx);
       const float4 v = *reinterpret_cast<const float4*>(p.o_part + ((int64_t)s * p.prows + row) * D + ch * 4);
       sum = fmaf(f, ml.y, sum);
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(256) ctx_combine_kernel(const CtxParams p) {
 #pragma unroll
     for (int k = 0; k < kTeams; ++k) {
       const float2 ml = ml_s[threadIdx.x + k * TPR];
-      if (ml.x == -INFINITY) continue;
+      if (ml.y == 0.f) continue;
       const float f = ex2_approx(ml.x - mx);
       const float4 v = acc_s[threadIdx.x + k * TPR];
       sum = fmaf(f, ml.y, sum);

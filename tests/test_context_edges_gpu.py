@@ -108,3 +108,27 @@ def test_fp16_weights_far_below_the_largest(cuda_lib, b, lq, d, gap):
     over = np.abs(got - ref) - tol
     assert over.max() <= 0, f"{got.flat[0]:.4e} instead of {ref.flat[0]:.4e}, bound {tol.flat[0]:.1e}"
     assert torch.equal(out[0, :lq], out[b - 1, :lq])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("b,lq,lkv,ls,h,hkv,d", [
+    (2, 2, 300, 0, 4, 2, 64),          # few rows, whole
+    (2, 2, 9000, 0, 4, 2, 128),        # few rows, cut
+    (2, 200, 300, 0, 2, 2, 64),        # many rows
+    (1, 200, 3000, 0, 2, 2, 128),      # many rows, cut
+    (2, 1, 7, 70000, 8, 2, 64),        # pooled, few rows
+    (33, 1, 257, 4200, 8, 2, 64),      # pooled in the tcgen05 kernel
+    (1, 10200, 1000, 0, 8, 4, 64),     # the last round's items cut
+])
+def test_a_query_that_is_nan_shows(cuda_lib, b, lq, lkv, ls, h, hkv, d, dtype):
+    """A NaN query gives NaN in its own row and head, whether the key list is cut or not, and changes nothing else."""
+    q, kv, sh = _make(52, b, lq, lkv, h, hkv, d, dtype, ls=ls)
+    ref = _call(q, kv, h, d, kv_heads=hkv, shared_kv=sh)
+    at = [(0, 0, 0), (b - 1, lq - 1, h - 1)]
+    for bq, i, hq in at:
+        q[bq, i, hq * d + 5] = float("nan")
+    out = _call(q, kv, h, d, kv_heads=hkv, shared_kv=sh)
+    for bq, i, hq in at:
+        assert out[bq, i, hq * d:(hq + 1) * d].isnan().all(), f"NaN query {bq, i, hq} is lost"
+        out[bq, i, hq * d:(hq + 1) * d] = ref[bq, i, hq * d:(hq + 1) * d]
+    assert torch.equal(out, ref)
