@@ -197,6 +197,13 @@ __device__ __forceinline__ Tile<kKeys> tile_of(const CtxParams& p, const Keys& k
   return t;
 }
 
+// Maximum of three, NaN where one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // One aligned 32-byte sector.
 __device__ __forceinline__ void st_32b(void* dst, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
@@ -510,8 +517,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
         for (int c = 0; c < kWords; ++c)
 #pragma unroll
           for (int e = 0; e < 32; e += 2)
-            mx[e / 2 & 3] = fmax3(mx[e / 2 & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
-        const float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+            mx[e / 2 & 3] = max3_nan(mx[e / 2 & 3], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+        const float rmax = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
         const float m_new = fmaxf(m, rmax);
         const bool upd = m_new > m + kRescaleThreshold<kFp16>;
         float alpha = 1.f;
@@ -519,7 +526,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
           alpha = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
           m = m_new;
         }
-        const float nm = m == -INFINITY ? 0.f : kLift<kFp16> - m;
+        // A score of NaN or +inf makes the whole row NaN, l with it. (exp2_poly2 does not pass NaN on: its clamp drops it.)
+        const float nm = !(rmax < INFINITY) ? NAN : m == -INFINITY ? 0.f : kLift<kFp16> - m;
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < kWords; ++c) {

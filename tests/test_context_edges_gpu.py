@@ -132,3 +132,21 @@ def test_a_query_that_is_nan_shows(cuda_lib, b, lq, lkv, ls, h, hkv, d, dtype):
         assert out[bq, i, hq * d:(hq + 1) * d].isnan().all(), f"NaN query {bq, i, hq} is lost"
         out[bq, i, hq * d:(hq + 1) * d] = ref[bq, i, hq * d:(hq + 1) * d]
     assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("lq,d", [(2, 64), (2, 128), (200, 64), (200, 128)])
+def test_a_valid_key_that_is_not_finite_shows(cuda_lib, lq, d, dtype):
+    """NaN in a valid key, or a score of +inf, makes the softmax NaN, wherever in a tile the key lies; the other batch
+    elements keep their bits."""
+    b, h, lkv = 3, 2, 150
+    q, kv, _ = _make(51, b, lq, lkv, h, h, d, dtype)
+    q[..., ::d] = 1.0
+    ref = _call(q, kv, h, d)
+    for bad in (float("nan"), float("inf")):
+        for key in (*range(64, 72), 3, 6, 15, 127, lkv - 1):
+            x = kv.clone()
+            x[1, key, 0] = bad                       # head 0 of batch element 1
+            out = _call(q, x, h, d)
+            assert out[1, :, :d].isnan().all(), f"{bad} at key {key} is lost"
+            assert torch.equal(out[1, :, d:], ref[1, :, d:]) and torch.equal(out[::2], ref[::2])
