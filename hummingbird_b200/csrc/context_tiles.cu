@@ -605,6 +605,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
       if (w + gridDim.x < total) load_q(w + gridDim.x);  // (the S MMAs of this unit are done)
       if (!first && !(ok = warp_wait(o_done, done++ & 1, abort_flag))) break;
       tc_fence_after();
+      // Nothing but scores of -inf: no weight. (exp2_poly2 gives them 2^-125 instead of 0, which shows only here.)
+      if (m == -INFINITY && l > 0.f) l = 0.f;
       const int gr = u.rt * 128 + row;
       const bool live = gr < u.rows;
       const CtxRow x = ctx_row(p, live ? gr : 0, u.g, u.b, part.pooled);

@@ -146,13 +146,14 @@ typedef struct HbContextArgs {
  *             eps) * q_weight, rounded to the 16-bit type as hb_head_rms_norm stores it).
  *   out       16-bit [batch, q_len, num_heads * head_dim] by strides; must not overlap the inputs.
  *   dtype     HB_BF16 or HB_FP16, for q, kv, shared_kv and out alike.
- * A row without a valid key is written as zeros; what lies at keys that are not valid (infinities, NaN) does not
- * reach the result. Scores, softmax statistics and sums are fp32; the weights p are rounded to the 16-bit type for
- * the product with v (relative error at most 2^-8 or 2^-11 each; in fp16 a weight below 2^-25 of the row's largest may
- * be off by 2^-36 of that instead), the sum of p is not; exponentials are good to 7.5e-5. head_dim 64 or 128; rows of q,
- * kv, shared_kv, out and their strides 16-byte aligned, workspace 32-byte; kv's batch stride 0, or one of its two
- * strides a multiple of the other; kv_len and shared_len at most 2^24; scale > 0. The result does not depend on
- * timing: the same call gives the same bits. Calls that may overlap on the GPU need workspaces of their own. */
+ * A row without a valid key, or whose valid scores are all -inf, is written as zeros; a NaN or +inf score of a valid
+ * key makes its row NaN; what lies at keys that are not valid (infinities, NaN) does not reach the result. Scores,
+ * softmax statistics and sums are fp32; the weights p are rounded to the 16-bit type for the product with v (relative
+ * error at most 2^-8 or 2^-11 each; in fp16 a weight below 2^-25 of the row's largest may be off by 2^-36 of that
+ * instead), the sum of p is not; exponentials are good to 7.5e-5. head_dim 64 or 128; rows of q, kv, shared_kv, out
+ * and their strides 16-byte aligned, workspace 32-byte; kv's batch stride 0, or one of its two strides a multiple of
+ * the other; kv_len and shared_len at most 2^24; scale > 0. The result does not depend on timing: the same call gives
+ * the same bits. Calls that may overlap on the GPU need workspaces of their own. */
 int hb_context_attn(const HbContextArgs* args, cudaStream_t stream);
 
 /* ---- band (sliding-window) differential attention (SAME-L decoder) --------------------------------- */

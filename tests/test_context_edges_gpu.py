@@ -150,3 +150,16 @@ def test_a_valid_key_that_is_not_finite_shows(cuda_lib, lq, d, dtype):
             out = _call(q, x, h, d)
             assert out[1, :, :d].isnan().all(), f"{bad} at key {key} is lost"
             assert torch.equal(out[1, :, d:], ref[1, :, d:]) and torch.equal(out[::2], ref[::2])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("b,lq,lkv,d", [(2, 2, 100, 64), (2, 2, 5000, 128), (2, 200, 100, 64), (2, 200, 100, 128),
+                                        (1, 200, 3000, 64)])
+def test_scores_of_minus_infinity(cuda_lib, b, lq, lkv, d, dtype):
+    """Keys of score -inf have weight 0; where every valid key has it there is no weight at all, and the row is zero."""
+    q, kv, _ = _make(53, b, lq, lkv, 1, 1, d, dtype)
+    q[..., 0] = 1.0
+    kv[..., 0] = -float("inf")
+    assert (_call(q, kv, 1, d) == 0).all()
+    kv[:, lkv // 2, 0] = 0.5
+    assert torch.equal(_call(q, kv, 1, d), kv[:, lkv // 2, d:][:, None].expand(b, lq, d))
