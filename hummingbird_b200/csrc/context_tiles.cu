@@ -35,6 +35,7 @@
 #include "context_attn.h"
 #include "launch_after.h"
 #include "hb_sm100.cuh"
+#include "short_wait.cuh"
 
 namespace hb {
 namespace {
@@ -126,21 +127,6 @@ __device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
       ::"r"(smem_u32(bar)), "r"(lead) : "memory");
 }
 
-// Bounded waits that end early once another role has given up. A try suspends the thread for a while by itself, so
-// the limit is far above any wait of a working kernel; the loop stays a few instructions long because it is inlined
-// into every hot path (a longer one, with a clock, cost the kernel its instruction cache).
-constexpr uint32_t kWaitTries = 1u << 24;
-template <int kSleepNs>
-__device__ __forceinline__ bool slow_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-#pragma unroll 1
-  for (uint32_t i = 0; i < kWaitTries && !*abort_flag; ++i) {
-    if (kSleepNs) __nanosleep(kSleepNs);
-    if (mbar_try_wait(bar, parity)) return true;
-  }
-  if (!*abort_flag) record_error(HB_ERR_TIMEOUT);
-  *abort_flag = 1;
-  return false;
-}
 // The producer runs ahead: between tries it leaves the issue slots to the softmax.
 __device__ __forceinline__ bool producer_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return mbar_try_wait(bar, parity) || slow_wait<200>(bar, parity, abort_flag);
