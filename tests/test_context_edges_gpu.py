@@ -163,3 +163,38 @@ def test_scores_of_minus_infinity(cuda_lib, b, lq, lkv, d, dtype):
     assert (_call(q, kv, 1, d) == 0).all()
     kv[:, lkv // 2, 0] = 0.5
     assert torch.equal(_call(q, kv, 1, d), kv[:, lkv // 2, d:][:, None].expand(b, lq, d))
+
+
+CUT_LAST_ROUND = [
+    # b, lq, lkv, heads, kv heads, head_dim: more row tiles than run at once, and a last round that leaves CTAs idle
+    (3, 3400, 1000, 8, 4, 64),    # 648 on 592: all of the last round is the last batch element's
+    (2, 2648, 2000, 16, 16, 64),  # 672
+    (5, 1630, 900, 5, 5, 128),    # 325 on 296
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("b,lq,lkv,h,hkv,d", CUT_LAST_ROUND)
+def test_last_round_with_lengths_masks_and_norm(cuda_lib, b, lq, lkv, h, hkv, d, dtype):
+    """The items of a last, partly filled round are cut along the keys: over lengths (cut units without keys, or with
+    fewer tiles than parts), masks, the query norm, shared states and several batch elements."""
+    ctas, items = (592 if d == 64 else 296), b * hkv * -(-lq * (h // hkv) // 128)
+    assert items > ctas and items % ctas
+    q, kv, sh = _make(60, b, lq, lkv, h, hkv, d, dtype, ls=100)
+    g = torch.Generator().manual_seed(61)
+    w = (1 + 0.1 * torch.randn(d, generator=g)).cuda()
+    rows = torch.cat([torch.arange(0, lq, 211), torch.arange(lq - 130, lq, 9)]).unique().cuda()
+    j = torch.arange(lkv, device="cuda")[None]
+    mask = (torch.rand(b, lkv, generator=g) < 0.5).cuda()
+    mask[-1, 150:] = False                       # the last element's later tiles hold no valid key
+    for last in (lkv, 100, 1, 0):
+        lens = torch.full((b,), lkv, dtype=torch.int32, device="cuda")
+        lens[-1], lens[0] = last, lkv - 37
+        for use_mask, shared in ((False, None), (True, None), (True, sh)):
+            valid = (j < lens[:, None]) & (mask if use_mask else True)
+            dirty = kv.masked_fill(~valid[..., None], float("nan"))
+            kw = dict(kv_heads=hkv, lens=lens, mask=mask if use_mask else None, q_weight=w, shared_kv=shared)
+            out = _call(q, dirty, h, d, **kw)
+            assert torch.isfinite(out).all()
+            _check(out[:, rows], q[:, rows], dirty, h, d, **kw)
+            assert torch.equal(_call(q, dirty, h, d, **kw), out)
