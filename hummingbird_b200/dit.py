@@ -115,7 +115,8 @@ class DiT:
             raise ValueError("qkv_quant='w8a8' needs glue='cuda' and one rank per batch group")
         if cfg.out_quant == "w8a8" and glue != "cuda":
             raise ValueError("out_quant='w8a8' needs glue='cuda'")
-        if cfg.num_heads % cfg.context_kv_heads or (cfg.cross_differential and cfg.cross_kv_heads is not None):
+        if cfg.context_kv_heads < 1 or cfg.num_heads % cfg.context_kv_heads \
+                or (cfg.cross_differential and cfg.cross_kv_heads is not None):
             raise ValueError("cross_kv_heads must divide num_heads and needs cross_differential=False")
         if (cfg.num_heads // 2) % self.world or self.t1 - self.t0 <= self.mem_rows:
             raise ValueError(f"a clip of {self.seq} tokens and {cfg.num_heads // 2} head pairs does not split "

@@ -38,3 +38,9 @@ def _worker(rank, world, split_batch, shared):
 def test_masked_cross_attention_over_ranks(world, split_batch, shared):
     """Each rank takes its batch rows of the mask; shared states go to all of them."""
     _run(_worker, world, split_batch, shared)
+
+
+@pytest.mark.parametrize("cfg", [dict(cross_kv_heads=0), dict(cross_kv_heads=-4), dict(cross_kv_heads=3)])
+def test_kv_heads_that_do_not_divide_the_heads_are_refused(cfg):
+    with pytest.raises(ValueError):
+        _dit(None, **cfg)
