@@ -131,19 +131,23 @@ def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, out_f
 
 
 class W4Linear:
-    """`nn.Linear` with weight `[out, in]` (the checkpoint layout, dit.py:34) and 4-bit weights: quantised once,
-    applied to the few rows of a conditioning vector. `act="silu"` takes the activation that follows along."""
+    """`nn.Linear` with weight `[out, in]` (the checkpoint layout, dit.py:34) and 4-bit weights: rounded to bf16 and
+    quantised once, applied to the few rows of a conditioning vector. `act="silu"` takes the activation that follows
+    along. fp16 inputs are taken and answered in fp16, all others in bf16."""
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, *, group: int = 128,
                  act: str | None = None):
         self.packed, self.scales = quantize_w4(weight.to(torch.bfloat16), group)
         self.bias = None if bias is None else bias.to(torch.bfloat16).contiguous()
+        self._bias_fp16 = None if bias is None else bias.to(torch.float16).contiguous()
         self.out_features, self.in_features = weight.shape
         self.group, self.act = group, act
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         if x.shape[-1] != self.in_features:
             raise ValueError(f"x must have {self.in_features} columns, got {tuple(x.shape)}")
-        x2 = x.reshape(-1, self.in_features).to(torch.bfloat16)
-        y = w4_linear(x2, self.packed, self.scales, self.out_features, self.group, self.bias, act=self.act)
+        fp16 = x.dtype == torch.float16
+        x2 = x.reshape(-1, self.in_features).to(torch.float16 if fp16 else torch.bfloat16)
+        y = w4_linear(x2, self.packed, self.scales, self.out_features, self.group,
+                      self._bias_fp16 if fp16 else self.bias, act=self.act)
         return y.reshape(*x.shape[:-1], self.out_features)

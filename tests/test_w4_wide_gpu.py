@@ -45,3 +45,22 @@ def test_two_tiles_of_outputs_to_a_cta(cuda_lib, m, n, k, group, act, with_bias,
     rest[1:-1, 3:3 + n] = 5.0
     assert (rest == 5.0).all()
     assert torch.equal(w4.w4_linear(x[:8], packed, scales, n, group, bias, act=act), got[:8].to(dtype))  # one tile a CTA
+
+
+def test_linear_class_keeps_fp16(cuda_lib):
+    """fp16 inputs go through the fp16 kernel with the bias in fp16 (values that bf16 would round), and come back so."""
+    from hummingbird_b200.w4 import W4Linear, dequantize_w4, w4_linear
+    g = torch.Generator(device="cuda").manual_seed(1)
+    weight, bias = torch.randn(96, 256, generator=g, device="cuda"), torch.randn(96, generator=g, device="cuda")
+    x = torch.randn(2, 3, 256, generator=g, device="cuda").to(FP16)
+    for b in (bias, None):
+        lin = W4Linear(weight, b, group=64)
+        y = lin(x)
+        w = dequantize_w4(lin.packed, lin.scales, 96, 256, 64).double()
+        ref = x.double() @ w.T + (0 if b is None else b.double())
+        mag = x.double().abs() @ w.abs().T + 4
+        assert y.dtype == FP16 and y.shape == (2, 3, 96)
+        assert ((y.double() - ref).abs() <= UNIT[FP16] * (ref.abs() + 4) * 1.01 + 257 * 2.0 ** -23 * mag).all()
+        bf = lin(x.to(BF16))
+        assert bf.dtype == BF16 and lin(x.float()).dtype == BF16
+        assert torch.equal(bf, w4_linear(x.to(BF16).view(6, 256), lin.packed, lin.scales, 96, 64, lin.bias).view(2, 3, 96))
