@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const uint32_t w = live ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + half * 8 + tid * 2)) : 0u;
+          const uint32_t w = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + half * 8 + tid * 2) : 0u;
           qf[mt][kk][half * 2 + hf] = w;
           const float2 f = T::unpack(w);
           ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) ctx_rows_kernel(const CtxParam
         for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const float2 w = __ldg(reinterpret_cast<const float2*>(p.q_w + kk * 16 + half * 8 + tid * 2));
+            const float2 w = *reinterpret_cast<const float2*>(p.q_w + kk * 16 + half * 8 + tid * 2);
             const float2 f = T::unpack(qf[mt][kk][half * 2 + hf]);
             qf[mt][kk][half * 2 + hf] = T::pack(f.x * inv * w.x, f.y * inv * w.y);
           }

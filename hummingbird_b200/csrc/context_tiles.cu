@@ -277,8 +277,10 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
   };
   // Up to here nothing but parameters was read, so this may run while the kernel before still does (a call among others
   // 20.5 -> 19.1 us at the 120 s clip's cross-attention). The launch beside the few-rows kernel does not wait for that
-  // one here: it was let in by a kernel that had waited itself.
-  if (!beside) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // one here: it was let in by a kernel that had waited itself, so all that it reads is in memory, and the fence keeps
+  // ordinary loads (lengths, masks, the norm's weights) from older lines of this SM's L1.
+  if (beside) __threadfence();
+  else asm volatile("griddepcontrol.wait;" ::: "memory");
   if (warp < 4) load_q(blockIdx.x);
   tc_fence_before();
   __syncthreads();
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
       if (p.q_w) {  // rounded to the input's type, as the norm pass that this replaces stores it
         float wv[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) wv[e] = __ldg(p.q_w + qch * 8 + e);
+        for (int e = 0; e < 8; ++e) wv[e] = p.q_w[qch * 8 + e];
 #pragma unroll 2
         for (int i = 0; i < kSteps; ++i) {
           uint4* at = reinterpret_cast<uint4*>(smem + (qch >> 3) * kQAtom + sw128_offset(qrow + i * kRowsPerStep, qch & 7));

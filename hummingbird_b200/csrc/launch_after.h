@@ -10,7 +10,9 @@ namespace hb {
 // (griddepcontrol.launch_dependents), or else when that one is done: its setup then costs no time of its own. A kernel
 // launched so reads and writes nothing but its parameters before griddepcontrol.wait, which returns when the one
 // before is complete with its memory visible, and allows the next one only after that; or it reads nothing that the
-// one before writes, was let in by a kernel that had waited itself, and waits before it ends.
+// one before writes, was let in by a kernel that had waited itself, and waits before it ends. What other kernels may have
+// written is read with ordinary loads or asynchronous copies, never with __ldg: that asks for memory that nothing writes
+// while the kernel lives, and the kernel lives before they are done.
 template <class... P, class... A>
 int launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
                  const A&... args) {

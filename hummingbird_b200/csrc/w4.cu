@@ -178,13 +178,13 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 6 : NT == 2 ? 4 : 3 - R
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) xv[t][w] = __ldg(reinterpret_cast<const uint4*>(xp[t] + 32 * w));
+          for (int w = 0; w < 4; ++w) xv[t][w] = *reinterpret_cast<const uint4*>(xp[t] + 32 * w);
       } else {  // the row's last block, where K is no multiple of 128
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            xv[t][w] = (i * kWarps + warp) * 128 + 32 * w < p.K ? __ldg(reinterpret_cast<const uint4*>(xp[t] + 32 * w))
+            xv[t][w] = (i * kWarps + warp) * 128 + 32 * w < p.K ? *reinterpret_cast<const uint4*>(xp[t] + 32 * w)
                                                                 : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll

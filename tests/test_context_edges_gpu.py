@@ -198,3 +198,40 @@ def test_last_round_with_lengths_masks_and_norm(cuda_lib, b, lq, lkv, h, hkv, d,
             assert torch.isfinite(out).all()
             _check(out[:, rows], q[:, rows], dirty, h, d, **kw)
             assert torch.equal(_call(q, dirty, h, d, **kw), out)
+
+
+def test_inputs_rewritten_in_place_before_every_call(cuda_lib):
+    """Kernels that start under the end of the one before read only what it leaves behind: queries, norm weights, lengths
+    and masks that the kernel right before each call rewrites, through both kernels, side by side, and W4 layers."""
+    from hummingbird_b200 import w4
+    shapes = [(4, 2, 300, 0, 4, 2, 64), (2, 200, 300, 0, 2, 2, 64), (33, 1, 257, 4200, 8, 2, 64), (2, 200, 300, 0, 2, 2, 128)]
+    for b, lq, lkv, ls, h, hkv, d in shapes:
+        qa, kv, sh = _make(70, b, lq, lkv, h, hkv, d, BF16, ls=ls)
+        qb, _, _ = _make(71, b, lq, 1, h, hkv, d, BF16)
+        g = torch.Generator().manual_seed(72)
+        sets = [(x, (1 + 0.3 * torch.randn(d, generator=g)).cuda(),
+                 torch.randint(1, lkv + 1, (b,), generator=g, dtype=torch.int32).cuda(),
+                 (torch.rand(b, lkv, generator=g) < 0.5).cuda()) for x in (qa, qb)]
+        live = [t.clone() for t in sets[0]]
+        one = lambda q, w, n, m: _call(q, kv, h, d, kv_heads=hkv, shared_kv=sh, q_weight=w, lens=n, mask=m)  # noqa: E731
+        refs = []
+        for s in sets:
+            refs.append(one(*s))
+            torch.cuda.synchronize()
+        outs = []
+        for turn in range(60):
+            for which, t in enumerate(live):     # one of them by the last kernel before the call, each in its turn
+                if which != turn % 4:
+                    t.copy_(sets[turn % 2][which])
+            live[turn % 4].copy_(sets[turn % 2][turn % 4])
+            outs.append(one(*live))
+        assert all(torch.equal(o, refs[i % 2]) for i, o in enumerate(outs))
+    packed, scales = w4.quantize_w4(torch.randn(2000, 1024, device="cuda").to(BF16), 128)
+    for m in (1, 9, 32):
+        x = torch.randn(m, 1024, device="cuda").to(BF16)
+        ref = w4.w4_linear(x, packed, scales, 2000, 128)
+        outs = []
+        for _ in range(60):
+            x.neg_()
+            outs.append(w4.w4_linear(x, packed, scales, 2000, 128))
+        assert all(torch.equal(o, ref if i % 2 else -ref) for i, o in enumerate(outs))
