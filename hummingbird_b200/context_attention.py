@@ -77,7 +77,8 @@ def _plan(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_ma
     if batch and q_len:
         n = ctypes.c_size_t(0)
         _lib.call("hb_context_workspace_bytes", batch, q_len, kv_len, shared_len, num_heads, kv_heads, head_dim,
-                  int(mask is not None or shared_mask is not None), ctypes.byref(n))
+                  int((mask is not None and kv_len > 0) or (shared_mask is not None and shared_len > 0)),
+                  ctypes.byref(n))
         need = n.value
     strides = (q.stride(0), q.stride(1), kv.stride(0), kv.stride(1), 0 if shared_kv is None else shared_kv.stride(0),
                0 if mask is None else mask.stride(0))
@@ -139,7 +140,8 @@ def _attend(q, shared_kv, kv, num_heads, head_dim, kv_heads, lens, mask, shared_
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     out_strides = out.stride()
     args = _ARGS.pack(q_at, kv_at, shared_at, 0 if lens is None else lens.data_ptr(),
-                      0 if mask is None else mask.data_ptr(), 0 if shared_mask is None else shared_mask.data_ptr(),
+                      mask.data_ptr() if mask is not None and sizes[2] else 0,  # (one without a state is none)
+                      shared_mask.data_ptr() if shared_mask is not None and sizes[3] else 0,
                       weight_at, out.data_ptr(), 0 if ws is None else ws.data_ptr(), *strides, out_strides[0],
                       out_strides[1], need, *sizes, eps, head_dim ** -0.5 if scale is None else scale)
     launch(device, "hb_context_attn", call, args)

@@ -235,3 +235,19 @@ def test_inputs_rewritten_in_place_before_every_call(cuda_lib):
             x.neg_()
             outs.append(w4.w4_linear(x, packed, scales, 2000, 128))
         assert all(torch.equal(o, ref if i % 2 else -ref) for i, o in enumerate(outs))
+
+
+@pytest.mark.parametrize("b,lq,ls,h,hkv,d", [(6, 1820, 25804, 8, 4, 128), (2, 3, 40, 2, 2, 64)])
+def test_masks_of_no_state(cuda_lib, b, lq, ls, h, hkv, d):
+    """A batch whose elements have no own states may still pass its (empty) mask: the call is that of none, workspace
+    included, however many shared states there are."""
+    q, kv, sh = _make(80, b, lq, 0, h, hkv, d, BF16, ls=ls)
+    mask = torch.ones(b, 0, dtype=torch.bool, device="cuda")
+    kw = dict(kv_heads=hkv, shared_kv=sh)
+    out = _call(q, kv, h, d, mask=mask, **kw)
+    assert torch.equal(out, _call(q, kv, h, d, **kw))
+    rows = torch.arange(0, lq, max(1, lq // 3)).cuda()
+    _check(out[:1, rows], q[:1, rows], kv[:1], h, d, **kw)
+    empty = _call(q[:, :3], kv, h, d, kv_heads=hkv, mask=mask, shared_kv=sh[:0],
+                  shared_mask=torch.ones(0, dtype=torch.bool, device="cuda"))
+    assert (empty == 0).all()
