@@ -20,8 +20,10 @@
 // Keys that are not valid: their scores are set to -inf, and in a tile that has some inside the tensor their V rows
 // are zeroed in shared memory (0 * NaN would reach O); tiles without any valid key are skipped by every role.
 //
-// Batch 2, 2,648 queries, 16 heads, 8,184 keys, D 64: 234 us, 760 TFLOP/s, 46 % of the measured bf16 rate; issue slots
-// 61 % used, MUFU 55 %, tensor pipe 36 %. At D 128 326 us, 1,090 TFLOP/s, 66 %.
+// Batch 2, 2,648 queries, 16 heads, 8,184 keys, D 64: 235 us (754 TFLOP/s, 46 % of cuBLAS's bf16 burst) in runs of a few
+// milliseconds, 262 us (677 TFLOP/s, 49 % of its sustained rate) in runs of a second, under the power cap. Issue slots 62 %
+// used, MUFU 55 %, tensor pipe 37 %: no pipe is full. D 128: 320 us (1,109 TFLOP/s) in short runs. The query norm stands
+// before a unit's first S: 21.5 us with it, 18.7 without, at 2 x 2,648 queries over a padded 257.
 //
 // Compiled as whole-program device code, as setmaxnreg needs; its status word is read by hb_device_status.
 #define HB_WHOLE_PROGRAM 1

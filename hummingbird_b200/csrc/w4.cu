@@ -15,8 +15,10 @@
 // One CTA takes 16 outputs (or 32); its four warps take every fourth block of 128 inputs, each through a ring of
 // asynchronous copies of its own, and merge through shared memory in warp order, so the result does not depend on
 // timing. x is read through L1 (it is the same few rows for every CTA).
-// One row, 16,384 x 8,192, group 128: 17.6 us, 3.9 TB/s, 60 % of the measured copy rate; unpacking bounds it (the
-// integer pipe is busy half of the time, instruction issue 60 %; 22 us with two logic operations to a nibble pair).
+// One row, 16,384 x 8,192, group 128: 17.4 us, 4.0 TB/s, 61 % of the measured copy rate. Nothing is full: issue 58 %,
+// integer pipe 50 % (22 us with two logic operations to a nibble pair); the longest stall is the wait for x, and 1,024 CTAs
+// on 888 places leave a short second round. 32 rows: 45.7 us, as long as a bf16 product takes (44.7): every CTA reads all
+// of x through L1, eight warps an SM wait for it (issue 31 %, tensor pipe 40 %).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -135,8 +137,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 6 : NT == 2 ? 4 : 3 - R
       for (int e = 0; e < 4; ++e) acc[q][t][e] = 0.f;
 
   // Each warp's blocks through a ring of its own: a lane copies what it reads of the weights itself, the scales are
-  // read by all. The integer pipe bounds this loop (seven operations to a word of eight weights), so all else is kept
-  // off it: pointers that step, stages by unrolling, rows past M read as row M - 1 (their columns are dropped).
+  // read by all. Integer operations are most of this loop (seven to a word of eight weights), so all else is kept off
+  // that pipe: pointers that step, stages by unrolling, rows past M read as row M - 1 (their columns are dropped).
   const uint8_t* wp =
       reinterpret_cast<const uint8_t*>(p.packed) + ((int64_t)tile * p.kblocks + warp) * 1024 + lane * 16;
   const uint8_t* sp = reinterpret_cast<const uint8_t*>(p.scales) +

@@ -95,7 +95,7 @@ def w4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, out_f
               bias: torch.Tensor | None = None, *, act: str | None = None,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """`act(x @ W^T + bias)` of bf16 or fp16 `x` `(M, K)` with the weights of `quantize_w4`: fp32 sums, one rounding
-    to x's type. `bias` `(N,)` of x's type; `act` "silu" or None ("none")."""
+    to x's type. `bias` `(N,)` of x's type; `act` "silu" or None ("none"). `out`, where given, overlaps no input."""
     key = (x.shape, x.stride(), x.dtype, packed.shape, packed.stride(), packed.dtype, scales.shape, scales.stride(),
            scales.dtype, out_features, group, act, None if bias is None else (bias.shape, bias.stride(), bias.dtype),
            None if out is None else (out.shape, out.stride(), out.dtype))
