@@ -22,8 +22,8 @@
 //
 // Batch 2, 2,648 queries, 16 heads, 8,184 keys, D 64: 235 us (754 TFLOP/s, 46 % of cuBLAS's bf16 burst) in runs of a few
 // milliseconds, 262 us (677 TFLOP/s, 49 % of its sustained rate) in runs of a second, under the power cap. Issue slots 62 %
-// used, MUFU 55 %, tensor pipe 37 %: no pipe is full. D 128: 320 us (1,109 TFLOP/s) in short runs. The query norm stands
-// before a unit's first S: 21.5 us with it, 18.7 without, at 2 x 2,648 queries over a padded 257.
+// used, MUFU 55 %, tensor pipe 37 %: no pipe is full. D 128: 320 to 338 us (1,109 to 1,050 TFLOP/s). The query norm stands
+// before a unit's first S: 20.4 us with it, 17.8 without, at 2 x 2,648 queries over a padded 257.
 //
 // Compiled as whole-program device code, as setmaxnreg needs; its status word is read by hb_device_status.
 #define HB_WHOLE_PROGRAM 1
@@ -249,10 +249,6 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 5) {
-    tmem_alloc(tmem_slot, L::kTmemCols);
-    tmem_relinquish();
-  }
   // Work unit w's queries, asynchronously into the shared-memory image (rows past the end as zeros): warp i its 32
   // rows, a row's PPR pieces by PPR consecutive lanes.
   constexpr int kRowsPerStep = 32 / PPR, kSteps = 32 / kRowsPerStep;
@@ -283,13 +279,19 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
   // ordinary loads (lengths, masks, the norm's weights) from older lines of this SM's L1.
   if (beside) __threadfence();
   else asm volatile("griddepcontrol.wait;" ::: "memory");
+  // TMEM is asked for only now: the kernel before may be anyone's (a library's product) and may let this one in before its
+  // own CTAs have theirs, so nothing is held while this one waits for it (and that call takes 18.1 us instead of 19.0).
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, L::kTmemCols);
+    tmem_relinquish();
+  }
   if (warp < 4) load_q(blockIdx.x);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // The merge, or the next early launch: they wait. Not before every CTA of this launch has its TMEM: a CTA of the next
-  // one keeps its columns while it waits for this launch, and must not hold what this one still asks for.
+  // The merge, or the next early launch: they wait. Not before every CTA of this launch has its TMEM, whatever the next
+  // one does with its own.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp >= 4) {

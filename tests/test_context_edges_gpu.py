@@ -251,3 +251,20 @@ def test_masks_of_no_state(cuda_lib, b, lq, ls, h, hkv, d):
     empty = _call(q[:, :3], kv, h, d, kv_heads=hkv, mask=mask, shared_kv=sh[:0],
                   shared_mask=torch.ones(0, dtype=torch.bool, device="cuda"))
     assert (empty == 0).all()
+
+
+@pytest.mark.parametrize("h,d", [(16, 64), (8, 128)])
+def test_right_behind_library_products(cuda_lib, h, d):
+    """As the DiT calls it: each call right behind the matrix product that makes its queries, which may let it in early."""
+    b, lq, w = 2, 1500, h * d
+    g = torch.Generator(device="cuda").manual_seed(90)
+    bf = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF16)  # noqa: E731
+    x, kv, proj = bf(b, lq, w), bf(b, 257, 2 * w), bf(4, w, w) / w ** 0.5
+    refs = []
+    for p in proj:
+        q = x @ p
+        torch.cuda.synchronize()
+        refs.append(_call(q, kv, h, d))
+        torch.cuda.synchronize()
+    outs = [_call(x @ proj[i % 4], kv, h, d) for i in range(40)]
+    assert all(torch.equal(o, refs[i % 4]) for i, o in enumerate(outs))
