@@ -268,3 +268,26 @@ def test_right_behind_library_products(cuda_lib, h, d):
         torch.cuda.synchronize()
     outs = [_call(x @ proj[i % 4], kv, h, d) for i in range(40)]
     assert all(torch.equal(o, refs[i % 4]) for i, o in enumerate(outs))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("lq,lkv,d", [(2, 250, 64), (2, 2040, 64), (2, 2040, 128), (200, 250, 64), (200, 2040, 64),
+                                      (200, 2040, 128)])
+def test_scores_in_the_ten_thousands(cuda_lib, lq, lkv, d, dtype):
+    """Scores around 60,000 in rising order, exact in fp32, within two of one another: the parts of a list have different
+    maxima, and a rounding of one against the weights that it stands for would show (half a unit of 87,000 is 2^-8). Bound:
+    roundings of the weights and of the output, 1e-4 for exponentials and fp32 sums."""
+    big = (d - 1) * 16 * 60 * 64 // d
+    q = torch.full((1, lq, d), 16.0 * 64 / d, dtype=dtype, device="cuda")
+    q[..., 0] = 2.0 ** -7
+    kv = torch.full((1, lkv, 2 * d), 60.0)
+    kv[..., 0] = torch.arange(lkv) // (lkv // 250)
+    kv[..., d:] = torch.randn(1, lkv, d, generator=torch.Generator().manual_seed(91))
+    kv = kv.to(dtype).cuda()
+    out = _call(q, kv, 1, d, scale=1.0).double()
+    s = (q.double() @ kv[..., :d].double().transpose(1, 2))
+    assert s.min() > big - 1 and s.max() < big + 3
+    p, v = torch.softmax(s, -1), kv[..., d:].double()
+    ref, a = p @ v, p @ v.abs()
+    u = UNIT[dtype]
+    assert ((out - ref).abs() <= u * (a + ref.abs()) * (1 + u) + 1e-4 * a).all(), (out - ref).abs().max().item()
