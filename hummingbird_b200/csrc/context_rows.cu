@@ -9,8 +9,8 @@
 // barrier between warps; m16n8k16 MMAs take the scores and P V, whose unused rows cost nothing that the bytes do
 // not cost already. The four warps of a CTA merge through shared memory, CTAs of a split key list through
 // (m, l, o) partials that ctx_combine_kernel joins in slot order, so results do not depend on timing.
-// Batch 8, one token, 32,768 keys, 16 heads over 4, D 64: 49 us with the merge, 5.5 TB/s, 84 % of the measured copy rate.
-// Two CTAs per SM hold 128 KB of copies in flight, where about 35 KB cover the memory's latency.
+// Batch 8, one token, 32,768 keys, 16 heads over 4, D 64: 49 us with the merge, 5.5 TB/s, 84 % of the measured copy
+// rate. Two CTAs per SM hold 128 KB of copies in flight, where about 35 KB cover the memory's latency.
 // Keys that the mask or the length leaves out are copied as zeros (their memory is not read) and their scores set
 // to -inf, so what lies there cannot reach the result; a row without keys gets zeros.
 #include <cuda_bf16.h>
@@ -30,9 +30,9 @@ constexpr int kChunkBytes = 8192;  // K and V of one chunk
 constexpr int kWarpBytes = kStages * kChunkBytes;
 constexpr int kRowsSmem = kWarps * kWarpBytes + kWarps * kStages * 4 + kWarps * 32 * 8;
 
-// kLift: all weights p <= 1 are multiplied by 2^kLift, so that small ones stay in the type's normal range for P V. fp16's
-// ends at 2^-14 (its subnormals at 2^-24): lifted, weights down to 2^-29 of the largest keep 11 bits, smaller ones are off
-// by at most 2^-40 of it.
+// kLift: all weights p <= 1 are multiplied by 2^kLift, so that small ones stay in the type's normal range for P V.
+// fp16's ends at 2^-14 (its subnormals at 2^-24): lifted, weights down to 2^-29 of the largest keep 11 bits, smaller
+// ones are off by at most 2^-40 of it.
 struct Bf16 {
   static constexpr float kLift = 0.f;
   static __device__ __forceinline__ float2 unpack(uint32_t w) { return {bf16_lo(w), bf16_hi(w)}; }
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(256) ctx_combine_kernel(const CtxParams p) {
 #pragma unroll 4
     for (int s = team; s < p.slots; s += kTeams) {
       const float2 ml = p.ml_part[(int64_t)s * p.prows + row];
-      if (ml.y == 0.f) continue;  // a part without keys left its sums unwritten (a NaN row's maximum is -inf too, its sum NaN)
+      if (ml.y == 0.f) continue;  // a part without keys (m = -inf, but a NaN row may have that too) left no sums
       const float f = ex2_approx(ml.x - mx);
       const float4 v = *reinterpret_cast<const float4*>(p.o_part + ((int64_t)s * p.prows + row) * D + ch * 4);
       sum = fmaf(f, ml.y, sum);

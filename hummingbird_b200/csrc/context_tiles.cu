@@ -8,8 +8,8 @@
 // scores 660 to 800 at D 64; and within a tile S, softmax and P V wait for one another, about as long again. So at D 64
 // four CTAs share an SM, as many as TMEM holds their S and O for (64 + 64 columns), and fill each other's waits. At
 // D 128 there is room for two, each with two buffers of S (2 x 64 + 128 columns): the next tile's S runs while this
-// one's softmax does. A lazy maximum (O is rescaled only when a row's maximum grows by more than 2^8, in fp16 2^4) keeps O in
-// TMEM, and a share of the exponentials goes to the FMA pipe (exp2_poly2).
+// one's softmax does. A lazy maximum (O is rescaled only when a row's maximum grows by more than 2^8, in fp16 2^4)
+// keeps O in TMEM, and a share of the exponentials goes to the FMA pipe (exp2_poly2).
 //
 // The grid is one round of CTAs; each walks its share of the units (tiles of rows), so barriers, TMEM and tensor maps
 // are set up once, K and V of the next unit are on their way early and its queries during the epilogue.
@@ -20,10 +20,10 @@
 // Keys that are not valid: their scores are set to -inf, and in a tile that has some inside the tensor their V rows
 // are zeroed in shared memory (0 * NaN would reach O); tiles without any valid key are skipped by every role.
 //
-// Batch 2, 2,648 queries, 16 heads, 8,184 keys, D 64: 235 us (754 TFLOP/s, 46 % of cuBLAS's bf16 burst) in runs of a few
-// milliseconds, 262 us (677 TFLOP/s, 49 % of its sustained rate) in runs of a second, under the power cap. Issue slots 62 %
-// used, MUFU 55 %, tensor pipe 37 %: no pipe is full. D 128: 320 to 338 us (1,109 to 1,050 TFLOP/s). The query norm stands
-// before a unit's first S: 20.4 us with it, 17.8 without, at 2 x 2,648 queries over a padded 257.
+// Batch 2, 2,648 queries, 16 heads, 8,184 keys, D 64: 235 us (754 TFLOP/s, 46 % of cuBLAS's bf16 burst) in runs of a
+// few milliseconds, 262 us (677 TFLOP/s, 49 % of its sustained rate) in runs of a second, under the power cap. Issue
+// slots 62 % used, MUFU 55 %, tensor pipe 37 %: no pipe is full. D 128: 320 to 338 us (1,109 to 1,050 TFLOP/s). The
+// query norm stands before a unit's first S: 20.4 us with it, 17.8 without, at 2 x 2,648 queries over a padded 257.
 //
 // Compiled as whole-program device code, as setmaxnreg needs; its status word is read by hb_device_status.
 #define HB_WHOLE_PROGRAM 1
@@ -44,11 +44,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kQAtom = 128 * 128;                // 128 rows of 128 bytes: 64 columns of a query tile
-// By how much (log2 units) a row's maximum may grow before O is rescaled, and what all weights are multiplied by (2^kLift)
-// so that small ones stay in P's normal range; P is at most 2^(kRescaleThreshold + kLift). bf16 has fp32's range. fp16's
-// normal range ends at 2^-14, its subnormal at 2^-24: lifted, weights down to 2^-25 of the largest keep 11 bits and
-// smaller ones are off by at most 2^-36 of it, 2^-11 in all over 2^25 keys (unlifted, 131,072 keys of weight 2^-25.2 beside
-// one of 1 were lost whole).
+// By how much (log2 units) a row's maximum may grow before O is rescaled, and what all weights are multiplied by
+// (2^kLift) so that small ones stay in P's normal range; P is at most 2^(kRescaleThreshold + kLift). bf16 has fp32's
+// range. fp16's normal range ends at 2^-14, its subnormal at 2^-24: lifted, weights down to 2^-25 of the largest keep
+// 11 bits and smaller ones are off by at most 2^-36 of it, 2^-11 in all over 2^25 keys (unlifted, 20,000 keys of weight
+// 2^-25.2 beside one of 1 were lost whole).
 template <bool kFp16>
 constexpr float kRescaleThreshold = kFp16 ? 4.f : 8.f;
 template <bool kFp16>
@@ -279,8 +279,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
   // ordinary loads (lengths, masks, the norm's weights) from older lines of this SM's L1.
   if (beside) __threadfence();
   else asm volatile("griddepcontrol.wait;" ::: "memory");
-  // TMEM is asked for only now: the kernel before may be anyone's (a library's product) and may let this one in before its
-  // own CTAs have theirs, so nothing is held while this one waits for it (and that call takes 18.1 us instead of 19.0).
+  // TMEM is asked for only now: the kernel before may be anyone's (a library's product) and may let this one in before
+  // its own CTAs have theirs, so nothing is held while this one waits for it (that call takes 18.1 us instead of 19.0).
   if (warp == 5) {
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
@@ -518,7 +518,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D>::kCtasPerSm)
           alpha = m == -INFINITY ? 0.f : ex2_approx(m - m_new);
           m = m_new;
         }
-        // A score of NaN or +inf makes the whole row NaN, l with it. (exp2_poly2 does not pass NaN on: its clamp drops it.)
+        // A score of NaN or +inf makes the whole row NaN, l with it. (exp2_poly2 does not pass NaN on: its clamp drops
+        // it.)
         const float nm = !(rmax < INFINITY) ? NAN : m == -INFINITY ? 0.f : kLift<kFp16> - m;
         float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
